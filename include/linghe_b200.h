@@ -353,6 +353,62 @@ int lh_fp8_gemm(const void* a, const void* b, const float* a_s, const float* b_s
 int lh_fp8_gemm_bb(const void* a, const void* b, const float* a_s, const float* b_s, void* c, int64_t M, int64_t N,
                    int64_t K, int block_size, int out_dtype, void* stream);
 
+/* ---- activations in eight bits between the linear layers -------------------------------
+ * No counterparts in the reference.  `codes` names the 8-bit format of a checkpoint: 1 = int8, 2 = e4m3
+ * (0 = none).  A checkpoint of a [M, n] tensor is its codes [M, n] and one float32 scale per 1x128 block,
+ * row-major [M, n/128] (the layout of lh_group_quant, whose outputs are a checkpoint of format 2):
+ *   scale = max(amax / top, 1e-30), top = 127 or 448;   code = nearest(x / scale), ties to even.
+ * A block with a NaN or an infinity has a NaN scale.  All pointers 16-byte aligned but those of scales, sums and
+ * per-row values. */
+
+/* The norm after a block, its gate and residual scale, the residual sum and the norm before the next block:
+ *   r_post = rsqrt(mean(o^2) + eps);  h = round(x + alpha * gate * (o * r_post * post));
+ *   r_pre = rsqrt(mean(h^2) + eps);   y = h * r_pre * pre         (h as rounded to `dtype`)
+ * x, o, h, y [M, n]; post, pre [n]; gate NULL or [G, n] with M a multiple of G, row i taking gate row i % G
+ * (G = 1: one value per channel; G = B for rows in [S, B] order: one per sample; G = M: one per element); all of
+ * `dtype`.  r_post, r_pre float32 [M].  n % 128 == 0, n <= 8192.
+ * codes != 0: also writes the checkpoints (oq, os) of o and (hq, hs) of h. */
+int lh_rmsnorm_pair_fwd(const void* x, const void* o, const void* post, const void* pre, const void* gate, int dtype,
+                        int64_t M, int64_t n, int64_t G, float alpha, float eps, int codes, void* h, void* y,
+                        float* r_post, float* r_pre, void* oq, float* os, void* hq, float* hs, void* stream);
+
+/* Gradient of the above.  dy, dh [M, n] of `dtype`: gradients of y and of h (dh may be NULL: zero).  o, h: the
+ * tensors of the forward pass (codes 0), or their checkpoints with scales os, hs.  r_post, r_pre from the forward pass.
+ * Writes dx = the gradient of x and of h's other use, dout = that of o [M, n]; dpost, dpre float32 [n]; dgate [G, n]
+ * of `dtype` (gate != NULL).  Sums over rows are float32 in a fixed order: equal calls give equal bits.
+ * scratch: lh_scratch_bytes("rmsnorm_pair_bwd", M, n) bytes.  M = 0 gives zero sums. */
+int lh_rmsnorm_pair_bwd(const void* dy, const void* dh, const void* o, const float* os, const void* h, const float* hs,
+                        const void* post, const void* pre, const void* gate, const float* r_post, const float* r_pre,
+                        int dtype, int64_t M, int64_t n, int64_t G, float alpha, int codes, void* dx, void* dout,
+                        float* dpost, float* dpre, void* dgate, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* SwiGLU that keeps an 8-bit checkpoint of its input: y [M,n] = silu(x1) * x2 [* w_row] of `dtype` and the
+ * checkpoint (q [M,2n], s [M,2n/128]) of x [M,2n].  codes 1 or 2; w NULL or [M] in w_dtype (LH_F32 / LH_BF16);
+ * n % 128 == 0. */
+int lh_silu_checkpoint_fwd(const void* x, const void* w, int dtype, int w_dtype, int codes, int64_t M, int64_t n,
+                           void* y, void* q, float* s, void* stream);
+
+/* Gradient from the checkpoint: g [M,n] and dx [M,2n] of `dtype`, dw [M] in w_dtype (w != NULL). */
+int lh_silu_checkpoint_bwd(const void* g, const void* q, const float* s, const void* w, int dtype, int w_dtype,
+                           int codes, int64_t M, int64_t n, void* dx, void* dw, void* stream);
+
+/* One float32 scale per row and int8 codes: x [M,K] of `dtype`, K % 16 == 0;
+ *   xs = x / max(smooth, 1e-30) (smooth float32 [K] or NULL);  s[m] = max(amax_k |xs| / 127, 1e-30);
+ *   q = nearest(xs / s), ties to even.  A row with a NaN or an infinity has a NaN scale. */
+int lh_token_quant_int8(const void* x, const float* smooth, int dtype, int64_t M, int64_t K, void* q, float* s,
+                        void* stream);
+
+/* c [M,N] = (sum_k a[m,k] * b[n,k]) * a_s[m] * b_s[n]: a [M,K], b [N,K] int8, a_s [M], b_s [N] float32, sums in
+ * 32-bit integers, exact.  K % 16 == 0, K <= 131056.  out_dtype LH_BF16 / LH_F16 / LH_F32. */
+int lh_int8_gemm(const void* a, const void* b, const float* a_s, const float* b_s, void* c, int64_t M, int64_t N,
+                 int64_t K, int out_dtype, void* stream);
+
+/* The two above in one call: c = x b^T with x [M,K] of `dtype` quantised per token into the workspaces
+ * q [M,K] (int8) and s [M] (float32), which hold the codes and scales afterwards.  The product starts while the
+ * quantiser still runs and waits for it on the device. */
+int lh_int8_linear(const void* x, const float* smooth, int dtype, const void* b, const float* b_s, void* q, float* s,
+                   void* c, int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

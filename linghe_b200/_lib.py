@@ -62,6 +62,13 @@ SIGNATURES = {
     "lh_silu_blockquant_bwd": (_i, [_p, _p, _i, _l, _l, _p, _p, _p, _p, _p, _i, _p]),
     "lh_batch_silu_blockquant_fwd": (_i, [_p, _p, _i, _i, _p, _i, _i, _l, _l, _p, _p, _p, _p, _i, _i, _p]),
     "lh_batch_silu_blockquant_bwd": (_i, [_p, _p, _p, _i, _i, _p, _i, _i, _l, _l, _p, _p, _p, _p, _p, _i, _p, _l, _p]),
+    "lh_rmsnorm_pair_fwd": (_i, [_p, _p, _p, _p, _p, _i, _l, _l, _l, _f, _f, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "lh_rmsnorm_pair_bwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _l, _l, _l, _f, _i, _p, _p, _p, _p, _p, _p, _l, _p]),
+    "lh_silu_checkpoint_fwd": (_i, [_p, _p, _i, _i, _i, _l, _l, _p, _p, _p, _p]),
+    "lh_silu_checkpoint_bwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _l, _l, _p, _p, _p]),
+    "lh_token_quant_int8": (_i, [_p, _p, _i, _l, _l, _p, _p, _p]),
+    "lh_int8_gemm": (_i, [_p, _p, _p, _p, _p, _l, _l, _l, _i, _p]),
+    "lh_int8_linear": (_i, [_p, _p, _i, _p, _p, _p, _p, _p, _l, _l, _l, _i, _p]),
 }
 
 _lock = threading.Lock()
@@ -115,7 +122,7 @@ def host():
 
 
 _DT_CODE = {torch.float8_e4m3fn: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3, torch.uint8: 4,
-            torch.int32: 5, torch.int64: 6}
+            torch.int32: 5, torch.int64: 6, torch.int8: 7}
 
 
 def empties(ref: torch.Tensor, *specs):
@@ -145,6 +152,26 @@ def itype_code(t: torch.Tensor) -> int:
         return _ITYPES[t.dtype]
     except KeyError:
         raise AssertionError(f"counts must be int32 or int64, got {t.dtype}") from None
+
+
+# 8-bit formats of an activation checkpoint, as the C ABI numbers them
+CHECKPOINTS = {None: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
+
+
+def checkpoint_code(dtype) -> int:
+    assert dtype in CHECKPOINTS, f"checkpoint must be torch.int8 or torch.float8_e4m3fn, got {dtype}"
+    return CHECKPOINTS[dtype]
+
+
+def check_same(ref: torch.Tensor, dtype, shape, **tensors):
+    """Each tensor (None is skipped) is contiguous, on the device of `ref`, of `dtype` and, where given, of `shape`."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        assert t.device == ref.device, f"{name} is on {t.device}, expected {ref.device}"
+        assert t.dtype == dtype, f"{name} is {t.dtype}, expected {dtype}"
+        assert shape is None or tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}"
+        assert t.is_contiguous(), f"{name} must be contiguous"
 
 
 def ptr(t):

@@ -204,6 +204,24 @@ int weighted_silu_fwd(const void* x, const void* w, int dtype, int w_dtype, int6
 int weighted_silu_bwd(const void* g, const void* x, const void* w, int dtype, int w_dtype, int64_t M, int64_t n,
                       void* dx, void* dw, cudaStream_t stream);
 
+int64_t pair_bwd_scratch(int64_t M, int64_t n);
+int pair_fwd(const void* x, const void* o, const void* post, const void* pre, const void* gate, int dtype, int64_t M, int64_t n,
+             int64_t G, float alpha, float eps, int codes, void* h, void* y, float* r_post, float* r_pre, void* oq, float* os,
+             void* hq, float* hs, cudaStream_t stream);
+int pair_bwd(const void* dy, const void* dh, const void* o, const float* os, const void* h, const float* hs, const void* post,
+             const void* pre, const void* gate, const float* r_post, const float* r_pre, int dtype, int64_t M, int64_t n, int64_t G,
+             float alpha, int codes, void* dx, void* dout, float* dpost, float* dpre, void* dgate, void* scratch,
+             int64_t scratch_bytes, cudaStream_t stream);
+int silu8_fwd(const void* x, const void* w, int dtype, int w_dtype, int codes, int64_t M, int64_t n, void* y, void* q, float* s,
+              cudaStream_t stream);
+int silu8_bwd(const void* g, const void* q, const float* s, const void* w, int dtype, int w_dtype, int codes, int64_t M, int64_t n,
+              void* dx, void* dw, cudaStream_t stream);
+int token_quant_int8(const void* x, const float* smooth, int dtype, int64_t M, int64_t K, void* q, float* s, cudaStream_t stream);
+int int8_gemm(const void* a, const void* b, const float* a_s, const float* b_s, void* c, int64_t M, int64_t N, int64_t K, int out_dtype,
+              bool dependent, cudaStream_t stream);
+int int8_linear(const void* x, const float* smooth, int dtype, const void* b, const float* b_s, void* q, float* s, void* c, int64_t M,
+                int64_t N, int64_t K, int out_dtype, cudaStream_t stream);
+
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // col_only_unit: column granularity the entry point accepts in output_mode 1 (transposed outputs
@@ -287,6 +305,7 @@ int64_t lh_scratch_bytes(const char* what, int64_t rows, int64_t cols) {
     if (!strcmp(what, "smooth_quant_bwd")) return smooth_bwd_scratch(cols);     // cols = n (half the row)
     if (!strcmp(what, "rmsnorm_bwd_static")) return 0;  // it carries its own
     if (!strcmp(what, "row_id_map")) return route_scratch_bytes(cols);          // cols = experts
+    if (!strcmp(what, "rmsnorm_pair_bwd")) return pair_bwd_scratch(rows, cols);
     if (!strcmp(what, "rmsnorm_gemm")) return router_gemm_scratch(rows, cols);   // rows = N, cols = K
     return -1;
 }
@@ -593,6 +612,45 @@ int lh_batch_silu_blockquant_bwd(const void* g, const void* x, const void* w, in
     if (int rc = tile_silu_bwd(g, x, w, w_dtype, dtype, counts, counts_type, E, R, n, dx_q, dx_s, dx_qt, dx_st, nullptr,
                                static_cast<float*>(scratch), round_scale, cs)) return rc;
     return dw_reduce(static_cast<const float*>(scratch), R, n / 128, dw, w_dtype, cs);
+}
+
+int lh_rmsnorm_pair_fwd(const void* x, const void* o, const void* post, const void* pre, const void* gate, int dtype, int64_t M,
+                        int64_t n, int64_t G, float alpha, float eps, int codes, void* h, void* y, float* r_post, float* r_pre,
+                        void* oq, float* os, void* hq, float* hs, void* stream) {
+    return pair_fwd(x, o, post, pre, gate, dtype, M, n, G, alpha, eps, codes, h, y, r_post, r_pre, oq, os, hq, hs,
+                    static_cast<cudaStream_t>(stream));
+}
+
+int lh_rmsnorm_pair_bwd(const void* dy, const void* dh, const void* o, const float* os, const void* h, const float* hs,
+                        const void* post, const void* pre, const void* gate, const float* r_post, const float* r_pre, int dtype,
+                        int64_t M, int64_t n, int64_t G, float alpha, int codes, void* dx, void* dout, float* dpost, float* dpre,
+                        void* dgate, void* scratch, int64_t scratch_bytes, void* stream) {
+    return pair_bwd(dy, dh, o, os, h, hs, post, pre, gate, r_post, r_pre, dtype, M, n, G, alpha, codes, dx, dout, dpost, dpre, dgate,
+                    scratch, scratch_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int lh_silu_checkpoint_fwd(const void* x, const void* w, int dtype, int w_dtype, int codes, int64_t M, int64_t n, void* y, void* q,
+                           float* s, void* stream) {
+    return silu8_fwd(x, w, dtype, w_dtype, codes, M, n, y, q, s, static_cast<cudaStream_t>(stream));
+}
+
+int lh_silu_checkpoint_bwd(const void* g, const void* q, const float* s, const void* w, int dtype, int w_dtype, int codes, int64_t M,
+                           int64_t n, void* dx, void* dw, void* stream) {
+    return silu8_bwd(g, q, s, w, dtype, w_dtype, codes, M, n, dx, dw, static_cast<cudaStream_t>(stream));
+}
+
+int lh_token_quant_int8(const void* x, const float* smooth, int dtype, int64_t M, int64_t K, void* q, float* s, void* stream) {
+    return token_quant_int8(x, smooth, dtype, M, K, q, s, static_cast<cudaStream_t>(stream));
+}
+
+int lh_int8_gemm(const void* a, const void* b, const float* a_s, const float* b_s, void* c, int64_t M, int64_t N, int64_t K,
+                 int out_dtype, void* stream) {
+    return int8_gemm(a, b, a_s, b_s, c, M, N, K, out_dtype, false, static_cast<cudaStream_t>(stream));
+}
+
+int lh_int8_linear(const void* x, const float* smooth, int dtype, const void* b, const float* b_s, void* q, float* s, void* c,
+                   int64_t M, int64_t N, int64_t K, int out_dtype, void* stream) {
+    return int8_linear(x, smooth, dtype, b, b_s, q, s, c, M, N, K, out_dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -24,7 +24,7 @@
 // L2 -> shared-memory traffic by a quarter, but leaves two partial buffers and 64 accumulator registers
 // per fold thread; measured level with 128 at 8192^3 and behind it at 4096^3, where 512 tiles on 148 SMs
 // quantise badly.  At 128 the kernel moves 32 KB per block and SM through L2, about 9.5 TB/s in all.
-#include "lh_common.cuh"
+#include "lh_umma.cuh"
 
 #include <type_traits>
 
@@ -50,16 +50,6 @@ static_assert(F_SMEM <= 232448, "shared memory");
 constexpr int F_SCALE_WARP = 2 + F_FOLD_WARPS;  // warp that stages the scales
 constexpr int F_THREADS = 32 * (F_SCALE_WARP + 1);
 
-enum : int { DEVERR_PART_WAIT = 5 };
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// K-major operand, rows of 128 bytes, 128-byte swizzle, groups of 8 rows 1024 bytes apart
-__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr) {
-    return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) |
-           (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
 // D f32, A and B e4m3 (format 0), both K-major, N = 128, M = 128
 constexpr uint32_t kIdescF8 = (1u << 4) | (uint32_t(FN >> 3) << 17) | (uint32_t(FM >> 4) << 24);
 
@@ -70,10 +60,6 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(kIdescF8), "r"(accumulate)
         : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
 }
 // 16 lanes x 32 columns in the accumulator-fragment layout: register 4 i + 2 hi + lo of thread t holds
 // lane (t / 4) + 8 hi, column 8 i + 2 (t % 4) + lo, counted from the address.  A thread then owns two
@@ -87,17 +73,6 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&v)[16]) 
         : "r"(taddr)
         : "memory");
 }
-// true in one lane of the (converged) warp, the same lane every time
-__device__ __forceinline__ bool elect_one() {
-    uint32_t pred;
-    asm volatile(
-        "{\n\t.reg .pred P;\n\t"
-        "elect.sync _|P, 0xffffffff;\n\t"
-        "selp.u32 %0, 1, 0, P;\n\t}"
-        : "=r"(pred));
-    return pred != 0;
-}
-
 struct Fp8GemmParams {
     const float* a_s;
     const float* b_s;

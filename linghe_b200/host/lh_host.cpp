@@ -131,16 +131,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> silu_and_block_quant_
 }
 
 // Several uninitialised tensors on the device of `ref` from one call: specs = [(shape, code), ...]
-// with code 0 e4m3, 1 float32, 2 bfloat16, 3 float16, 4 uint8, 5 int32, 6 int64.  One
+// with code 0 e4m3, 1 float32, 2 bfloat16, 3 float16, 4 uint8, 5 int32, 6 int64, 7 int8.  One
 // Python -> C++ transition instead of one per torch.empty.
 std::vector<at::Tensor> empty_many(const at::Tensor& ref, const std::vector<std::pair<std::vector<int64_t>, int>>& specs) {
-    static const at::ScalarType kinds[] = {at::kFloat8_e4m3fn, at::kFloat, at::kBFloat16, at::kHalf, at::kByte, at::kInt, at::kLong};
+    static const at::ScalarType kinds[] = {at::kFloat8_e4m3fn, at::kFloat, at::kBFloat16, at::kHalf, at::kByte, at::kInt, at::kLong, at::kChar};
     if (!ref.is_cuda()) throw std::runtime_error("linghe_b200 runs on CUDA tensors only (no CPU fallback)");
     std::vector<at::Tensor> out;
     out.reserve(specs.size());
     const c10::cuda::OptionalCUDAGuard guard(ref.device());
     for (const auto& sp : specs) {
-        if (sp.second < 0 || sp.second > 6) raise_assert("empty_many: unknown dtype code");
+        if (sp.second < 0 || sp.second > 7) raise_assert("empty_many: unknown dtype code");
         out.push_back(at::empty(sp.first, ref.options().dtype(kinds[sp.second])));
     }
     return out;

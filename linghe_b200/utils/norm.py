@@ -198,3 +198,82 @@ def triton_rms_norm_and_smooth_quant_forward(
               M, N, float(eps), _lib.ptr(out), _lib.ptr(scale), _lib.ptr(rms) if output_rms else 0, _lib.ptr(maxs),
               _lib.ptr(scratch), nbytes, int(bool(round_scale)))
     return out, scale, maxs, rms
+
+
+def _gate_rows(gate, x):
+    """Rows G of a gate whose shape is that of the last dimensions of x (leading ones aside); 0 without a gate."""
+    if gate is None:
+        return 0
+    shape = tuple(gate.shape)
+    while len(shape) > 1 and shape[0] == 1:
+        shape = shape[1:]
+    assert 1 <= len(shape) <= x.dim() and shape == tuple(x.shape[x.dim() - len(shape):]), (
+        f"gate has shape {tuple(gate.shape)}, expected that of the last dimensions of x {tuple(x.shape)}")
+    return gate.numel() // x.shape[-1]
+
+
+def rms_norm_pair_forward(x, o, post_weight, pre_weight, gate=None, residual_scale=1.0, eps=1e-6, checkpoint=None):
+    """The norm after a block, its gate and residual scale, the residual sum and the norm before the next block:
+
+        h = x + residual_scale * gate * RMSNorm(o) * post_weight;   y = RMSNorm(h) * pre_weight
+
+    x (the residual stream) and o (the block's output) [M, n] or [S, B, n]; n % 128 == 0, n <= 8192.  `gate`: None, or
+    a tensor of the shape of x's last dimensions -- [n] one value per channel, [B, n] one per sample of an [S, B, n]
+    batch, the shape of x one per element.  The second norm is that of h as rounded to its type.
+    `checkpoint` (torch.int8 or torch.float8_e4m3fn): also write 8-bit checkpoints of o and h, which
+    rms_norm_pair_backward takes in their place.
+    Returns (h like x, y like x, rms_post f32 [M], rms_pre f32 [M], saved): the rms are 1/rms per row of o and of h;
+    saved is None or (o_q [.., n], o_scale f32 [M, n/128], h_q, h_scale).  Upstream has no such operator."""
+    M, n = _rows_cols(x)
+    assert n > 0 and n % 128 == 0 and n <= 8192
+    codes = _lib.checkpoint_code(checkpoint)
+    _lib.check_same(x, x.dtype, x.shape, x=x, o=o)
+    _lib.check_same(x, x.dtype, (n,), post_weight=post_weight, pre_weight=pre_weight)
+    _lib.check_same(x, x.dtype, None, gate=gate)
+    G = _gate_rows(gate, x)
+    shape = tuple(x.shape)
+    specs = [(shape, x.dtype), (shape, x.dtype), ((M,), torch.float32), ((M,), torch.float32)]
+    if codes:
+        specs += [(shape, checkpoint), ((M, n // 128), torch.float32)] * 2
+    outs = _lib.empties(x, *specs)
+    h, y, rms_post, rms_pre = outs[:4]
+    saved = tuple(outs[4:]) if codes else None
+    oq, os_, hq, hs = saved or (None, None, None, None)
+    _lib.call("lh_rmsnorm_pair_fwd", x, _lib.ptr(x), _lib.ptr(o), _lib.ptr(post_weight), _lib.ptr(pre_weight), _lib.ptr(gate),
+              _lib.dtype_code(x), M, n, G, float(residual_scale), float(eps), codes, _lib.ptr(h), _lib.ptr(y), _lib.ptr(rms_post),
+              _lib.ptr(rms_pre), _lib.ptr(oq), _lib.ptr(os_), _lib.ptr(hq), _lib.ptr(hs))
+    return h, y, rms_post, rms_pre, saved
+
+
+def rms_norm_pair_backward(grad_y, grad_h, o, h, post_weight, pre_weight, rms_post, rms_pre, gate=None, residual_scale=1.0,
+                           o_scale=None, h_scale=None):
+    """Gradient of rms_norm_pair_forward.  grad_h (the gradient that reaches h from its other use, the residual stream
+    of the next block) may be None.  o and h are the forward pass's tensors, or with o_scale and h_scale their 8-bit
+    checkpoints (`saved` of the forward pass; the outputs of triton_group_quant are a checkpoint too).
+    Returns (dx, do like grad_y, dpost f32 [n], dpre f32 [n], dgate like gate or None)."""
+    M, n = _rows_cols(grad_y)
+    assert n > 0 and n % 128 == 0 and n <= 8192
+    dt = grad_y.dtype
+    _lib.check_same(grad_y, dt, grad_y.shape, grad_y=grad_y, grad_h=grad_h)
+    assert (o_scale is None) == (h_scale is None), "o_scale and h_scale are given together"
+    codes = 0 if o_scale is None else _lib.checkpoint_code(o.dtype)
+    assert o_scale is None or codes, "o and h with scales are 8-bit checkpoints"
+    _lib.check_same(grad_y, dt if o_scale is None else o.dtype, grad_y.shape, o=o, h=h)
+    _lib.check_same(grad_y, torch.float32, (M, n // 128), o_scale=o_scale, h_scale=h_scale)
+    _lib.check_same(grad_y, dt, (n,), post_weight=post_weight, pre_weight=pre_weight)
+    _lib.check_same(grad_y, torch.float32, (M,), rms_post=rms_post, rms_pre=rms_pre)
+    _lib.check_same(grad_y, dt, None, gate=gate)
+    G = _gate_rows(gate, grad_y)
+    shape = tuple(grad_y.shape)
+    nbytes = _lib.scratch_bytes("rmsnorm_pair_bwd", M, n)
+    specs = [(shape, dt), (shape, dt), ((n,), torch.float32), ((n,), torch.float32), ((nbytes,), torch.uint8)]
+    if gate is not None:
+        specs.append((tuple(gate.shape), dt))
+    outs = _lib.empties(grad_y, *specs)
+    dx, do, dpost, dpre, scratch = outs[:5]
+    dgate = outs[5] if gate is not None else None
+    _lib.call("lh_rmsnorm_pair_bwd", grad_y, _lib.ptr(grad_y), _lib.ptr(grad_h), _lib.ptr(o), _lib.ptr(o_scale), _lib.ptr(h),
+              _lib.ptr(h_scale), _lib.ptr(post_weight), _lib.ptr(pre_weight), _lib.ptr(gate), _lib.ptr(rms_post), _lib.ptr(rms_pre),
+              _lib.dtype_code(grad_y), M, n, G, float(residual_scale), codes, _lib.ptr(dx), _lib.ptr(do), _lib.ptr(dpost),
+              _lib.ptr(dpre), _lib.ptr(dgate), _lib.ptr(scratch), nbytes)
+    return dx, do, dpost, dpre, dgate

@@ -294,3 +294,42 @@ def triton_batch_weighted_silu_and_smooth_quant_backward(g, x, weight, counts, s
               _lib.itype_code(counts), n_expert, M, n, s, _lib.ptr(dx), _lib.ptr(dx_scale), _lib.ptr(dw),
               _lib.ptr(transpose_dx), _lib.ptr(transpose_dx_scale), int(bool(round_scale)), int(bool(reverse)))
     return dx, dx_scale, dw, transpose_dx, transpose_dx_scale
+
+
+def silu_and_checkpoint_forward(x, weight=None, checkpoint=torch.int8):
+    """y = silu(x1) * x2 [* weight] for x = [x1 | x2] [M, 2n], and an 8-bit checkpoint of x that the backward pass
+    takes in its place: int8 or e4m3 codes with one float32 scale per 1x128 block.  `weight`: float32 or bf16 [M], one
+    value per row (a routing weight).  n % 128 == 0.  Upstream has no such operator: its SwiGLU saves x.
+    Returns (y [M, n] x.dtype, x_q [M, 2n], x_scale f32 [M, 2n/128])."""
+    M, N = x.shape
+    assert N > 0 and N % 256 == 0
+    codes = _lib.checkpoint_code(checkpoint)
+    assert codes, "checkpoint must be torch.int8 or torch.float8_e4m3fn"
+    _lib.check_same(x, x.dtype, None, x=x)
+    if weight is not None:
+        _lib.check_same(x, weight.dtype, (M,), weight=weight)
+    y, x_q, x_scale = _lib.empties(x, ((M, N // 2), x.dtype), ((M, N), checkpoint), ((M, N // 128), torch.float32))
+    _lib.call("lh_silu_checkpoint_fwd", x, _lib.ptr(x), _lib.ptr(weight), _lib.dtype_code(x),
+              _lib.dtype_code(weight) if weight is not None else _lib.F32, codes, M, N // 2, _lib.ptr(y), _lib.ptr(x_q),
+              _lib.ptr(x_scale))
+    return y, x_q, x_scale
+
+
+def silu_and_checkpoint_backward(g, x_q, x_scale, weight=None):
+    """Gradient of silu_and_checkpoint_forward from the checkpoint of x: g [M, n] -> (dx [M, 2n] g.dtype, dw like
+    weight or None).  Any row-major 1x128 codes of x will do, triton_group_quant's among them."""
+    M, N = x_q.shape
+    assert N > 0 and N % 256 == 0
+    codes = _lib.checkpoint_code(x_q.dtype)
+    _lib.check_same(g, g.dtype, (M, N // 2), g=g)
+    _lib.check_same(g, x_q.dtype, None, x_q=x_q)
+    _lib.check_same(g, torch.float32, (M, N // 128), x_scale=x_scale)
+    specs = [((M, N), g.dtype)]
+    if weight is not None:
+        _lib.check_same(g, weight.dtype, (M,), weight=weight)
+        specs.append(((M,), weight.dtype))
+    outs = _lib.empties(g, *specs)
+    dx, dw = outs[0], outs[1] if weight is not None else None
+    _lib.call("lh_silu_checkpoint_bwd", g, _lib.ptr(g), _lib.ptr(x_q), _lib.ptr(x_scale), _lib.ptr(weight), _lib.dtype_code(g),
+              _lib.dtype_code(weight) if weight is not None else _lib.F32, codes, M, N // 2, _lib.ptr(dx), _lib.ptr(dw))
+    return dx, dw
