@@ -358,6 +358,12 @@ __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wa
 // make generic-proxy shared-memory writes visible to the async proxy (bulk stores)
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Programmatic dependent launch: a kernel launched with the attribute may start while the one before it in the stream still
+// runs, once all of that one's CTAs have said so or ended; grid_wait() returns when that one is complete and its writes are
+// visible (at once in a kernel launched without the attribute).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <int ID, int N>
 __device__ __forceinline__ void named_bar() {
     asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");

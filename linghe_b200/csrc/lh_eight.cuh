@@ -8,6 +8,8 @@
 #pragma once
 #include "lh_common.cuh"
 
+#include <type_traits>
+
 namespace lh {
 
 enum : int { CODES_NONE = 0, CODES_INT8 = 1, CODES_E4M3 = 2 };
@@ -64,11 +66,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+// max(|a|, |b|, |c|), a NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float amax_pairs(const float2* v) {   // four pairs
-    float m = max_nan(fabsf(v[0].x), fabsf(v[0].y));
-#pragma unroll
-    for (int i = 1; i < 4; ++i) m = max_nan(m, max_nan(fabsf(v[i].x), fabsf(v[i].y)));
-    return m;
+    const float a = max3_nan(v[0].x, v[0].y, v[1].x), b = max3_nan(v[1].y, v[2].x, v[2].y);
+    return max3_nan(max3_nan(a, b, v[3].x), v[3].y, 0.f);
 }
 
 // RN(a / 127) by the sequence of div448 (checked against division for every mantissa)
@@ -141,11 +147,59 @@ __device__ __forceinline__ void decode8(uint2 w, float scale, float2* v) {
     for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], splat2(scale));
 }
 
-// maximum over the 16 lanes that hold one block of 128 elements
-__device__ __forceinline__ float block_amax(float a) {
+// ---- a lane's share of a row: 32 bytes of a 16-bit type (16 elements) or of float32 (8) --------
+template <typename T> constexpr int kSpan = 32 / int(sizeof(T));
+
+template <typename T>
+struct Lane {
+    static constexpr int V = kSpan<T> / 8;
+    Vec8<T> v[V];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
-    return a;
-}
+        for (int i = 0; i < V; ++i) v[i].zero();
+    }
+    // wide: p is 32-byte aligned, else 16
+    __device__ __forceinline__ void load(const uint8_t* p, bool wide) {
+        if (wide) {
+            uint4 a, b;
+            ld_global_256(p, a, b);
+            put(a, b);
+        } else {
+            put(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + 16));
+        }
+    }
+    __device__ __forceinline__ void put(const uint4& a, const uint4& b) {
+        constexpr int H = V - 1, J = 4 * (2 - V);
+        v[0].w[0] = a.x; v[0].w[1] = a.y; v[0].w[2] = a.z; v[0].w[3] = a.w;
+        v[H].w[J] = b.x; v[H].w[J + 1] = b.y; v[H].w[J + 2] = b.z; v[H].w[J + 3] = b.w;
+    }
+    __device__ __forceinline__ void store(uint8_t* p, bool wide) const {
+        constexpr int H = V - 1, J = 4 * (2 - V);
+        const uint4 a = make_uint4(v[0].w[0], v[0].w[1], v[0].w[2], v[0].w[3]), b = make_uint4(v[H].w[J], v[H].w[J + 1], v[H].w[J + 2], v[H].w[J + 3]);
+        if (wide) {
+            st_global_256(p, a, b);
+        } else {
+            *reinterpret_cast<uint4*>(p) = a;
+            *reinterpret_cast<uint4*>(p + 16) = b;
+        }
+    }
+};
+template <int V>
+struct Codes {                     // V times eight codes
+    uint2 w[V];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if constexpr (V == 2) {
+            const uint4 q = *reinterpret_cast<const uint4*>(p);
+            w[0] = make_uint2(q.x, q.y);
+            w[1] = make_uint2(q.z, q.w);
+        } else {
+            w[0] = *reinterpret_cast<const uint2*>(p);
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* p) const {
+        if constexpr (V == 2) *reinterpret_cast<uint4*>(p) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
+        else *reinterpret_cast<uint2*>(p) = w[0];
+    }
+};
 
 }  // namespace lh

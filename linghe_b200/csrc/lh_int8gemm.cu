@@ -19,87 +19,90 @@ namespace {
 
 constexpr int64_t kInt8MaxK = 131071 / 16 * 16;
 
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // ---- token-wise quantiser ---------------------------------------------------------------------
-// A team of 1, 2, 4 or 8 warps takes a row, a lane 8 consecutive elements at a time.  Rows of up to 32 elements
-// per lane (HOLD) stay in registers between the maximum and the codes, longer ones are read again, from L2.
-constexpr int kTokThreads = 256, kTokVec = 4;
+// A team of warps takes a row, a lane 32 bytes of it.  Rows that 16 warps hold that way (HOLD: 8192 elements of a 16-bit
+// type, 4096 of float32) stay in registers between the maximum and the codes, longer ones are walked twice, the second
+// time through L2.  Small registers, so that six rows of 4096 are in flight on an SM: that is what it waits for.
+constexpr int kTokWarps = 16;
 
 struct TokenParams {
     const uint8_t* x;
     const float* smooth;
     int64_t M;
-    int K;
+    int K, wide;
     uint8_t* q;
     float* s;
 };
 
-template <typename T, bool HOLD>
-__global__ void __launch_bounds__(kTokThreads) token_quant_kernel(const TokenParams p, int team) {
-    __shared__ float part[kTokThreads / 32];
-    constexpr int ES = sizeof(T);
-    grid_go();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, teams = kTokThreads / 32 / team;
-    const int64_t row = int64_t(blockIdx.x) * teams + warp / team;
-    const bool any = row < p.M;
-    const uint8_t* x = p.x + (any ? row : 0) * p.K * ES;
-    const int first = (warp % team) * 256 + lane * 8, stride = team * 256;
+// the elements at column c over max(smooth, 1e-30)
+template <typename T>
+__device__ __forceinline__ void smoothed(const Lane<T>& x, const float* smooth, int c, float2 (&e)[Lane<T>::V][4]) {
+#pragma unroll
+    for (int v = 0; v < Lane<T>::V; ++v) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[v][i] = x.v[v].get(i);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float4 m = *reinterpret_cast<const float4*>(smooth + c + 8 * v + 4 * h);
+            float2 &lo = e[v][2 * h], &hi = e[v][2 * h + 1];
+            lo = make_float2(__fdiv_rn(lo.x, max_nan(m.x, kScaleFloor)), __fdiv_rn(lo.y, max_nan(m.y, kScaleFloor)));
+            hi = make_float2(__fdiv_rn(hi.x, max_nan(m.z, kScaleFloor)), __fdiv_rn(hi.y, max_nan(m.w, kScaleFloor)));
+        }
+    }
+}
 
-    // element group at column c, smoothed
-    auto load = [&](int c, float2* v) {
-        Vec8<T> w;
-        w.load(x + int64_t(c) * ES);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = w.get(i);
-        if (p.smooth) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float4 m = *reinterpret_cast<const float4*>(p.smooth + c + 4 * h);
-                v[2 * h] = make_float2(__fdiv_rn(v[2 * h].x, max_nan(m.x, kScaleFloor)), __fdiv_rn(v[2 * h].y, max_nan(m.y, kScaleFloor)));
-                v[2 * h + 1] = make_float2(__fdiv_rn(v[2 * h + 1].x, max_nan(m.z, kScaleFloor)), __fdiv_rn(v[2 * h + 1].y, max_nan(m.w, kScaleFloor)));
-            }
-        }
-    };
+template <typename T, bool HOLD, bool SMOOTH>
+__global__ void __launch_bounds__(32 * kTokWarps, SMOOTH ? 2 : 3) token_quant_kernel(const TokenParams p, int team) {
+    constexpr int ES = sizeof(T), SPAN = kSpan<T>, V = Lane<T>::V;
+    __shared__ float part[kTokWarps];
+    grid_go();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, teams = (blockDim.x >> 5) / team;
+    const int64_t row = int64_t(blockIdx.x) * teams + warp / team;
+    const bool any = row < p.M, wide = p.wide != 0;
+    const uint8_t* x = p.x + (any ? row : 0) * p.K * ES;
+    const int first = (warp % team * 32 + lane) * SPAN, stride = team * 32 * SPAN;
     float amax = 0.f;
-    float2 held[HOLD ? kTokVec : 1][4];
-    if constexpr (HOLD) {
+    Lane<T> w;
+    float2 e[SMOOTH ? V : 1][4];      // the quotients by the smoothing factors are kept, values are unpacked again
+    for (int c = first; any && c < p.K; c += stride) {          // HOLD: once at most
+        w.load(x + int64_t(c) * ES, wide);
+        if constexpr (SMOOTH) smoothed(w, p.smooth, c, e);
 #pragma unroll
-        for (int k = 0; k < kTokVec; ++k) {
+        for (int v = 0; v < V; ++v) {
+            if constexpr (!SMOOTH)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) held[k][i] = make_float2(0.f, 0.f);
-            if (any && first + k * stride < p.K) load(first + k * stride, held[k]);
+                for (int i = 0; i < 4; ++i) e[0][i] = w.v[v].get(i);
+            amax = max_nan(amax, amax_pairs(e[SMOOTH ? v : 0]));
         }
-#pragma unroll
-        for (int k = 0; k < kTokVec; ++k) amax = max_nan(amax, amax_pairs(held[k]));
-    } else {
-        for (int c = first; any && c < p.K; c += stride) {
-            load(c, held[0]);
-            amax = max_nan(amax, amax_pairs(held[0]));
-        }
+        if (HOLD) break;
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
     if (team > 1) {
         if (lane == 0) part[warp] = amax;
         __syncthreads();
-        for (int i = 0; i < team; ++i) amax = max_nan(amax, part[warp / team * team + i]);
+        amax = part[warp / team * team + min(lane & 15, team - 1)];
+#pragma unroll
+        for (int d = 8; d >= 1; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
     }
     if (!any) return;
-    const float scale = code_scale<CODES_INT8>(amax);
-    const Divisor d(scale);
-    if (lane == 0 && warp % team == 0) p.s[row] = scale;
-    uint8_t* q = p.q + row * p.K;
-    if constexpr (HOLD) {
-#pragma unroll
-        for (int k = 0; k < kTokVec; ++k)
-            if (first + k * stride < p.K) *reinterpret_cast<uint2*>(q + first + k * stride) = encode8<CODES_INT8>(held[k], d);
-    } else {
-        for (int c = first; c < p.K; c += stride) {
-            load(c, held[0]);
-            *reinterpret_cast<uint2*>(q + c) = encode8<CODES_INT8>(held[0], d);
+    const Divisor d(code_scale<CODES_INT8>(amax));
+    if (lane == 0 && warp % team == 0) p.s[row] = d.s;
+    for (int c = first; c < p.K; c += stride) {
+        if constexpr (!HOLD) {
+            w.load(x + int64_t(c) * ES, wide);
+            if constexpr (SMOOTH) smoothed(w, p.smooth, c, e);
         }
+        Codes<V> q;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if constexpr (!SMOOTH)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[0][i] = w.v[v].get(i);
+            q.w[v] = encode8<CODES_INT8>(e[SMOOTH ? v : 0], d);
+        }
+        q.store(p.q + row * p.K + c);
+        if (HOLD) break;
     }
 }
 
@@ -643,17 +646,23 @@ int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
     return go(std::integral_constant<int, 128>{});
 }
 
-int token_launch(const TokenParams& p, int dtype, cudaStream_t stream) {
-    int team = 1;
-    while (team < 8 && team * 512 < p.K) team *= 2;
-    const int teams = kTokThreads / 32 / team;
+int token_launch(TokenParams p, int dtype, cudaStream_t stream) {
+    p.wide = (int64_t(p.K) * (dtype == LH_F32 ? 4 : 2)) % 32 == 0 && aligned(p.x, 32);
+    const int span = dtype == LH_F32 ? 8 : 16;
+    const int64_t warps = ceil_div(p.K, 32 * span);
+    const bool hold = warps <= kTokWarps;
+    const int team = hold ? int(warps) : kTokWarps, teams = std::max(1, 4 / team);
     const int64_t grid = ceil_div(p.M, teams);
     if (grid > 0x7fffffff) return fail_arg("token_quant_int8: too many rows");
-    const bool hold = p.K <= team * 256 * kTokVec;
-    auto go = [&](auto kern) { return launch("token_quant_kernel", kern, unsigned(grid), kTokThreads, 0, 1, false, stream, p, team); };
-    if (dtype == LH_BF16) return hold ? go(token_quant_kernel<__nv_bfloat16, true>) : go(token_quant_kernel<__nv_bfloat16, false>);
-    if (dtype == LH_F16) return hold ? go(token_quant_kernel<__half, true>) : go(token_quant_kernel<__half, false>);
-    return hold ? go(token_quant_kernel<float, true>) : go(token_quant_kernel<float, false>);
+    auto go = [&](auto kern) { return launch("token_quant_kernel", kern, unsigned(grid), 32u * team * teams, 0, 1, false, stream, p, team); };
+    auto with = [&](auto type) {
+        using T = decltype(type);
+        if (p.smooth) return hold ? go(token_quant_kernel<T, true, true>) : go(token_quant_kernel<T, false, true>);
+        return hold ? go(token_quant_kernel<T, true, false>) : go(token_quant_kernel<T, false, false>);
+    };
+    if (dtype == LH_BF16) return with(__nv_bfloat16{});
+    if (dtype == LH_F16) return with(__half{});
+    return with(float{});
 }
 
 int token_check(const char* what, const void* x, const float* smooth, int dtype, int64_t M, int64_t K, const void* q, const float* s) {

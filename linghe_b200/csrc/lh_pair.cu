@@ -11,10 +11,7 @@
 //   dpre = sum dy * hn;   dpost = sum dp * on;   dgate = sum alpha * dh * on * post
 //
 // Both are one pass over HBM: 8 bytes per element forward (16-bit types), 12 backward, 10 with o and h
-// kept as 8-bit codes.  What has to be waited for is the row: two sums over it, one after the other, so
-// a row's tensors are brought to shared memory by bulk copies several rows ahead of the row being
-// worked on, and a thread keeps the columns it owns (the 8-element vectors t and t + NT of a row) for the
-// whole walk: gamma and the gradient sums of those columns stay in its registers.
+// kept as 8-bit codes.  What has to be waited for is the row: two sums over it, one after the other.
 #include "lh_eight.cuh"
 
 #include <algorithm>
@@ -28,7 +25,7 @@ constexpr int kPairMaxN = 8192;
 constexpr int kPairMaxThreads = kPairMaxN / 16;
 constexpr int kPairMaxStages = 4;
 constexpr int kPairSmem = 227 * 1024;      // shared memory of an SM that CTAs can ask for
-constexpr int kPairSlack = 1536;           // per CTA: static shared memory, what the system reserves, rounding
+constexpr int kPairSlack = 5120;           // per CTA: static shared memory, what the system reserves, rounding
 
 struct PairParams {
     const uint8_t *x, *o, *post, *pre, *gate;   // forward: x, o.  backward: o, h (values or codes)
@@ -36,7 +33,7 @@ struct PairParams {
     const float *os_in, *hs_in;                 // scales of the codes of o and h, [M, n / 128]
     int64_t M, G;                               // gate: G rows, row i takes gate row i % G
     int n;
-    int stages;
+    int stages, wide;
     float alpha, eps, inv_n;
     uint8_t *h, *y, *dx, *dout;
     float *r_post, *r_pre;
@@ -46,150 +43,113 @@ struct PairParams {
     uint8_t* dgate;
 };
 
-// Sum over the CTA.  buf has a place for each of 16 warps, those of absent warps zeroed; it is written
+// Sum over the CTA.  buf has a place for each of W warps, those of absent warps zeroed; it is written
 // again only behind another barrier of the caller.
+template <int W = 16>
 __device__ __forceinline__ float cta_sum(float v, float* buf) {
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
     __syncthreads();
-    float4 s[4];
+    v = buf[threadIdx.x & (W - 1)];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = reinterpret_cast<const float4*>(buf)[i];
-    float r = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r += (s[i].x + s[i].y) + (s[i].z + s[i].w);
-    return r;
+    for (int d = W / 2; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    return v;
 }
 
-// the codes of one block of 128 elements (16 lanes, eight elements each) and its scale; every lane of a warp comes here
-template <int CK>
-__device__ __forceinline__ void put_codes(const float2* e, bool live, uint8_t* q, float* scales, int64_t row, int n, int col) {
-    const float scale = code_scale<CK>(block_amax(amax_pairs(e)));
-    if (live) {     // blocks do not straddle the end of a row: n is a multiple of 128
-        *reinterpret_cast<uint2*>(q + row * n + col) = encode8<CK>(e, Divisor(scale));
-        if ((threadIdx.x & 15) == 0) scales[row * (n >> 7) + (col >> 7)] = scale;
-    }
-}
-
-enum : int { GATE_NONE = 0, GATE_ROW = 1, GATE_ROWS = 2 };
+enum : int { GATE_NONE = 0, GATE_ROW = 1, GATE_GROUPS = 2, GATE_EACH = 3 };   // gate rows: none, one, fewer than rows, as many as rows
 
 // ---- forward ---------------------------------------------------------------------------------
-// A gate of several rows is brought in with the row; where there is one row of it or none, alpha * gate * post is
-// one float32 coefficient per column.
-template <typename T, int CK, bool ROWS>
-__global__ void __launch_bounds__(kPairMaxThreads, sizeof(T) == 2 ? 2 : 1) pair_fwd_kernel(const PairParams p) {
-    extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ uint64_t full[kPairMaxStages];
-    __shared__ __align__(16) float sum_o[16], sum_h[16];
-    constexpr int ES = sizeof(T), NTEN = ROWS ? 3 : 2;
-    const int t = threadIdx.x, nt = blockDim.x, S = p.stages;
-    const uint32_t row_bytes = uint32_t(p.n) * ES, stage_bytes = NTEN * row_bytes;
-    const int64_t step = gridDim.x;
+// One CTA per row, a thread 32 consecutive bytes of it in registers, every load of the row asked for at once: with
+// 64 registers 1024 threads are resident, so four rows of 4096 are on their way to an SM while others are normalised
+// or stored.  Coefficients (the same for every row) come from L1 and L2: with the row where registers allow it (16-bit
+// types without checkpoints, 85 us; 88 where they are fetched when wanted), behind the sums elsewhere (with int8
+// checkpoints 122 us, 155 - 175 the other way).
+// Measured at 16384 x 4096, bf16: 85 us (97 % of the measured copy bandwidth).  A persistent walk fed by bulk copies through a
+// shared-memory ring took 92 - 102 us whatever its depth, order of rows, rows per step or cache hints, and 4.2 us
+// instead of 3.2 for 16 rows.
 
-    auto fetch = [&](int64_t row, int s) {
-        uint8_t* dst = ring + size_t(s) * stage_bytes;
-        mbar_expect_tx(&full[s], stage_bytes);
-        bulk_g2s(dst, p.o + row * row_bytes, row_bytes, &full[s]);
-        bulk_g2s(dst + row_bytes, p.x + row * row_bytes, row_bytes, &full[s]);
-        if (ROWS) bulk_g2s(dst + 2 * row_bytes, p.gate + (row % p.G) * row_bytes, row_bytes, &full[s]);
-    };
-    if (t == 0) {
-        for (int s = 0; s < S; ++s) mbar_init(&full[s], 1);
-        mbar_fence_init();
-        for (int s = 0; s < S && blockIdx.x + s * step < p.M; ++s) fetch(blockIdx.x + s * step, s);
-    }
-    if (t < 16) sum_o[t] = sum_h[t] = 0.f;
-
-    const int col[2] = {t * 8, (t + nt) * 8};
-    const bool live[2] = {col[0] < p.n, col[1] < p.n};
-    Vec8<T> pre[2];
-    float2 coef[8];      // alpha * post [* gate]
+// the codes of one block of 128 elements (16 / V lanes, 8 V elements each) and its scale; every lane of a warp comes here
+template <int CK, typename T>
+__device__ __forceinline__ void put_codes(const Lane<T>& d, bool live, uint8_t* q, float* scales, int64_t row, int n, int col) {
+    constexpr int V = Lane<T>::V;
+    float2 e[V][4];
+    float amax = 0.f;
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-        Vec8<T> w, g;
-        w.zero(); g.zero(); pre[v].zero();
-        if (live[v]) {
-            w.load(p.post + col[v] * ES);
-            if (!ROWS && p.gate) g.load(p.gate + col[v] * ES);
-            if (ES == 2) pre[v].load(p.pre + col[v] * ES);
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[v][i] = d.v[v].get(i);
+        amax = max_nan(amax, amax_pairs(e[v]));
+    }
+#pragma unroll
+    for (int m = 8 / V; m >= 1; m >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+    if (live) {     // blocks do not straddle the end of a row: n is a multiple of 128
+        const Divisor div(code_scale<CK>(amax));
+        Codes<V> c;
+#pragma unroll
+        for (int v = 0; v < V; ++v) c.w[v] = encode8<CK>(e[v], div);
+        c.store(q + row * n + col);
+        if ((threadIdx.x & (16 / V - 1)) == 0) scales[row * (n >> 7) + (col >> 7)] = div.s;
+    }
+}
+
+template <typename T, int CK>
+__global__ void __launch_bounds__(kPairMaxN * sizeof(T) / 32, sizeof(T) == 2 ? 2 : 1) pair_fwd_kernel(const PairParams p) {
+    constexpr int ES = sizeof(T), V = Lane<T>::V, W = 32 / V;
+    constexpr bool EARLY = ES == 2 && CK == CODES_NONE;
+    __shared__ float sum_o[W], sum_h[W];
+    const int t = threadIdx.x, col = t * 8 * V;
+    const bool live = col < p.n, wide = p.wide != 0;
+    const int64_t row_bytes = int64_t(p.n) * ES, row = blockIdx.x, at = row * row_bytes + col * ES;
+    Lane<T> o, x, post, pre, gate;
+    o.zero(); x.zero(); post.zero(); pre.zero(); gate.zero();
+    if (live) {
+        o.load(p.o + at, wide);
+        x.load(p.x + at, wide);
+        if (p.gate && (EARLY || p.G > 1)) gate.load(p.gate + (uint32_t(row) % uint32_t(p.G)) * row_bytes + col * ES, wide);   // fewer than 2^31 rows
+        if (EARLY) {
+            post.load(p.post + col * ES, wide);
+            pre.load(p.pre + col * ES, wide);
         }
+    }
+    if (t < W) sum_o[t] = sum_h[t] = 0.f;
+    __syncthreads();
+    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = fma2(o.v[v].get(i), o.v[v].get(i), acc);
+    if constexpr (CK != CODES_NONE) put_codes<CK>(o, live, p.oq, p.os, row, p.n, col);
+    const float r_post = rsqrtf(fmaf(cta_sum<W>(acc.x + acc.y, sum_o), p.inv_n, p.eps));
+    const float scaled = r_post * p.alpha;
+    if (!EARLY && live) {
+        post.load(p.post + col * ES, wide);
+        if (p.gate && p.G == 1) gate.load(p.gate + col * ES, wide);
+    }
+    acc = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            coef[4 * v + i] = mul2(w.get(i), splat2(p.alpha));
-            if (!ROWS && p.gate) coef[4 * v + i] = mul2(coef[4 * v + i], g.get(i));
+            float2 w = post.v[v].get(i);
+            if (p.gate) w = mul2(w, gate.v[v].get(i));
+            x.v[v].set(i, fma2(mul2(o.v[v].get(i), splat2(scaled)), w, x.v[v].get(i)));      // h, as it is stored
+            acc = fma2(x.v[v].get(i), x.v[v].get(i), acc);
         }
+    if (!live) acc = make_float2(0.f, 0.f);        // of a row without a finite norm, 0 * r_post is not 0
+    if (live) x.store(p.h + at, wide);
+    if constexpr (CK != CODES_NONE) put_codes<CK>(x, live, p.hq, p.hs, row, p.n, col);
+    const float r_pre = rsqrtf(fmaf(cta_sum<W>(acc.x + acc.y, sum_h), p.inv_n, p.eps));
+    if (t == 0) {
+        p.r_post[row] = r_post;
+        p.r_pre[row] = r_pre;
     }
-    __syncthreads();
-
-    bool dead = false;
-    int s = 0;
-    uint32_t phase = 0;
-    for (int64_t row = blockIdx.x; row < p.M; row += step) {
-        mbar_wait_or_mark<true>(&full[s], phase, DEVERR_FULL_WAIT, dead);
-        const uint8_t* so = ring + size_t(s) * stage_bytes;
-        float2 acc = make_float2(0.f, 0.f);
+    if (!EARLY && live) pre.load(p.pre + col * ES, wide);
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            Vec8<T> o;
-            o.zero();
-            if (live[v]) o.load(so + col[v] * ES);
-            float2 e[4];
+    for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[i] = o.get(i);
-                acc = fma2(e[i], e[i], acc);
-            }
-            if constexpr (CK != CODES_NONE) put_codes<CK>(e, live[v], p.oq, p.os, row, p.n, col[v]);
-        }
-        const float rp = __frsqrt_rn(fmaf(cta_sum(acc.x + acc.y, sum_o), p.inv_n, p.eps));
-
-        Vec8<T> h[2];
-        acc = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            h[v].zero();
-            if (live[v]) {
-                Vec8<T> x, o, g;
-                o.load(so + col[v] * ES);
-                x.load(so + row_bytes + col[v] * ES);
-                if (ROWS) g.load(so + 2 * row_bytes + col[v] * ES);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float2 q = mul2(o.get(i), splat2(rp));
-                    if (ROWS) q = mul2(q, g.get(i));
-                    h[v].set(i, fma2(q, coef[4 * v + i], x.get(i)));
-                }
-                h[v].store(p.h + row * row_bytes + col[v] * ES);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc = fma2(h[v].get(i), h[v].get(i), acc);
-        }
-        const float rh = __frsqrt_rn(fmaf(cta_sum(acc.x + acc.y, sum_h), p.inv_n, p.eps));
-        // behind that barrier every thread has read the stage
-        if (t == 0) {
-            if (row + S * step < p.M) fetch(row + S * step, s);
-            p.r_post[row] = rp;
-            p.r_pre[row] = rh;
-        }
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            if (live[v]) {
-                Vec8<T> y, w;
-                if (ES == 2) w = pre[v]; else w.load(p.pre + col[v] * ES);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y.set(i, mul2(mul2(h[v].get(i), splat2(rh)), w.get(i)));
-                y.store(p.y + row * row_bytes + col[v] * ES);
-            }
-            if constexpr (CK != CODES_NONE) {
-                float2 e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = h[v].get(i);
-                put_codes<CK>(e, live[v], p.hq, p.hs, row, p.n, col[v]);
-            }
-        }
-        if (++s == S) { s = 0; phase ^= 1u; }
-    }
+        for (int i = 0; i < 4; ++i) x.v[v].set(i, mul2(mul2(x.v[v].get(i), splat2(r_pre)), pre.v[v].get(i)));
+    if (live) x.store(p.y + at, wide);
 }
 
 // ---- backward --------------------------------------------------------------------------------
@@ -200,7 +160,9 @@ __global__ void __launch_bounds__(kPairMaxThreads, sizeof(T) == 2 ? 2 : 1) pair_
 //
 // B = sum dh * on is the one sum behind two gradients: dgate = alpha * post * B over the gate's group, and
 // dpost = alpha * sum over the groups of gate * B.  With one gate row or none the CTAs keep B alone (and the
-// sum for dpre), the reduction forms both; with several rows dpost has sums of its own.
+// sum for dpre), the reduction forms both; with several rows B starts again with every group, and dpost's sums, which
+// grow at the end of a group only, stay in shared memory.  Where every row has a gate row of its own that comes in with
+// the row, dgate is written row by row and B's place taken by dpost's sum.
 __host__ __device__ __forceinline__ int64_t pair_first(int64_t b, int64_t grid, int64_t M) {
     const int64_t q = M / grid, r = M % grid;
     return b * q + (b < r ? b : r);
@@ -209,205 +171,363 @@ __host__ __device__ __forceinline__ int64_t pair_first(int64_t b, int64_t grid, 
 // scratch: [grid][PART_ROWS][n] float32
 enum : int { PART_PRE = 0, PART_POST = 1, PART_HEAD = 2, PART_TAIL = 3, PART_ROWS = 4 };   // PART_POST: B itself with one gate row or none
 
+// Eight elements of o or h as they lie in shared memory: values, or codes that a block's scale makes values of.
+template <typename T, int CK>
+struct Kept {
+    uint2 w;
+    __device__ __forceinline__ void load(const uint8_t* p, int col) { w = *reinterpret_cast<const uint2*>(p + col); }
+    __device__ __forceinline__ void get(float2* e) const {
+        decode4<CK>(w.x, e[0], e[1]);
+        decode4<CK>(w.y, e[2], e[3]);
+    }
+};
+template <typename T>
+struct Kept<T, CODES_NONE> {
+    Vec8<T> w;
+    __device__ __forceinline__ void load(const uint8_t* p, int col) { w.load(p + col * int(sizeof(T))); }
+    __device__ __forceinline__ void get(float2* e) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = w.get(i);
+    }
+};
+
+__device__ __forceinline__ void copy4_async(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// global -> shared bulk copy of what no other kernel reads soon
+__device__ __forceinline__ void bulk_once(void* dst_smem, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+                     smem_u32(dst_smem)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Sums over the CTA of two values.  buf: a place for each of 16 warps and value, those of absent warps zeroed.
+__device__ __forceinline__ float2 cta_sum2(float a, float b, float* buf) {
+    const bool up = (threadIdx.x & 16) != 0;          // the halves of a warp take a value each after the first exchange
+    float v = up ? b : a;
+    v += __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if ((threadIdx.x & 15) == 0) buf[(threadIdx.x & 16) + (threadIdx.x >> 5)] = v;
+    __syncthreads();
+    v = buf[threadIdx.x & 31];
+#pragma unroll
+    for (int d = 8; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    const float o = __shfl_xor_sync(0xffffffffu, v, 16);
+    return up ? make_float2(o, v) : make_float2(v, o);
+}
+
+// A row passes three times through the registers: (1) sum t * hn, (2) dx, the sums over rows, u and sum u * on,
+// (3) do.  The two sums of a row are joined with its neighbours': between two barriers a CTA does (3) of row i, (2) of
+// row i + 1 and (1) of row i + 2, and the barrier exchanges the sums of the latter two.  That is one barrier and one
+// reduction's latency per row, with 16 warps on an SM (128 registers a thread) to hide it.  Rows come in by bulk copies,
+// their 1/rms and the scales of their codes by 4-byte copies two rows further ahead.
 template <typename T, int CK, int GATE>
 __global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const PairParams p) {
     extern __shared__ __align__(128) uint8_t ring[];
+    constexpr int NB = kPairMaxN / 128, SC = 2 * NB + 2, DEPTH = kPairMaxStages + 2;
     __shared__ uint64_t full[kPairMaxStages];
-    __shared__ __align__(16) float sum_h[16], sum_o[16];
-    constexpr bool ROWS = GATE == GATE_ROWS;
+    __shared__ float sums[2][32];
+    __shared__ float scal[DEPTH][SC];        // scales of o, of h, 1/rms of o, of h
+    constexpr bool GROUPS = GATE == GATE_GROUPS, EACH = GATE == GATE_EACH;
+    constexpr int V = 2;           // vectors of a thread in a row; one (64 registers, twice the warps) measured a quarter slower
     constexpr int ES = sizeof(T), CS = CK == CODES_NONE ? ES : 1;   // bytes of an element of dy / of o and h
-    const int t = threadIdx.x, nt = blockDim.x, S = p.stages;
+    const int t = threadIdx.x, nt = blockDim.x, S = p.stages, nb = p.n >> 7;
     const uint32_t row_bytes = uint32_t(p.n) * ES, code_bytes = uint32_t(p.n) * CS;
     const bool has_dh = p.dh != nullptr;
-    // a stage: dy | o | h | gate row (if the gate has several) | dh (if given)
-    const uint32_t off_o = row_bytes, off_h = off_o + code_bytes, off_g = off_h + code_bytes, off_dh = off_g + (ROWS ? row_bytes : 0u),
+    // a stage: dy | o | h | gate row (if every row has one) | dh (if given)
+    const uint32_t off_o = row_bytes, off_h = off_o + code_bytes, off_g = off_h + code_bytes, off_dh = off_g + (EACH ? row_bytes : 0u),
                    stage_bytes = off_dh + (has_dh ? row_bytes : 0u);
-    const int64_t G = ROWS ? p.G : 1, R = p.M / G;
-    const int64_t begin = pair_first(blockIdx.x, gridDim.x, p.M), end = pair_first(blockIdx.x + 1, gridDim.x, p.M);
+    const int G = GROUPS ? int(p.G) : 1, R = int(p.M) / G;          // fewer than 2^31 rows
+    const int begin = int(pair_first(blockIdx.x, gridDim.x, p.M)), end = int(pair_first(blockIdx.x + 1, gridDim.x, p.M));
 
-    auto fetch = [&](int64_t j, int s) {
-        const int64_t g = ROWS ? j / R : 0, row = ROWS ? g + (j - g * R) * G : j;
+    // a position, its gate row and its row; one step on costs no division
+    struct At { int j, g, left, row; };
+    auto start = [&](int j) {
+        At a{j, 0, 0, j};
+        if (GROUPS) {
+            a.g = j / R;
+            const int k = j - a.g * R;
+            a.left = R - k;
+            a.row = a.g + k * G;
+        }
+        return a;
+    };
+    auto advance = [&](At& a) {
+        ++a.j;
+        if (!GROUPS) ++a.row;
+        else if (--a.left == 0) { ++a.g; a.left = R; a.row = a.g; }
+        else a.row += G;
+    };
+    __shared__ At ahead;           // the position to be fetched next; thread 0 alone uses it
+    auto fetch = [&](int s) {
+        const int64_t row = ahead.row;
+        uint64_t policy;             // its lines go first when L2 needs room: 4 % at 16384 x 4096
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         uint8_t* dst = ring + size_t(s) * stage_bytes;
         mbar_expect_tx(&full[s], stage_bytes);
-        bulk_g2s(dst, p.dy + row * row_bytes, row_bytes, &full[s]);
-        bulk_g2s(dst + off_h, p.hsrc + row * code_bytes, code_bytes, &full[s]);
-        bulk_g2s(dst + off_o, p.o + row * code_bytes, code_bytes, &full[s]);
-        if (has_dh) bulk_g2s(dst + off_dh, p.dh + row * row_bytes, row_bytes, &full[s]);
-        if (ROWS) bulk_g2s(dst + off_g, p.gate + g * row_bytes, row_bytes, &full[s]);
+        bulk_once(dst, p.dy + row * row_bytes, row_bytes, &full[s], policy);
+        bulk_once(dst + off_h, p.hsrc + row * code_bytes, code_bytes, &full[s], policy);
+        bulk_once(dst + off_o, p.o + row * code_bytes, code_bytes, &full[s], policy);
+        if (has_dh) bulk_once(dst + off_dh, p.dh + row * row_bytes, row_bytes, &full[s], policy);
+        if (EACH) bulk_once(dst + off_g, p.gate + row * row_bytes, row_bytes, &full[s], policy);
+        advance(ahead);
+    };
+    // one group of 4-byte copies per row, an empty one past the last
+    const int nsc = CK == CODES_NONE ? 2 : 2 * nb + 2;               // fewer than threads
+    At sc_at = start(begin);
+    int sc_slot = 0;
+    auto fetch_scalars = [&]() {
+        if (sc_at.j < end && t < nsc) {
+            const int k = CK == CODES_NONE ? t + 2 * nb : t;
+            const float* src = k < nb ? p.os_in + int64_t(sc_at.row) * nb + k : k < 2 * nb ? p.hs_in + int64_t(sc_at.row) * nb + (k - nb)
+                               : k == 2 * nb ? p.r_post + sc_at.row : p.r_pre + sc_at.row;
+            copy4_async(&scal[sc_slot][k], src);
+        }
+        copies_commit();
+        advance(sc_at);
+        if (++sc_slot == DEPTH) sc_slot = 0;
     };
     if (t == 0) {
         for (int s = 0; s < S; ++s) mbar_init(&full[s], 1);
         mbar_fence_init();
-        for (int s = 0; s < S && begin + s < end; ++s) fetch(begin + s, s);
+        ahead = start(begin);
+        for (int s = 0; s < S && begin + s < end; ++s) fetch(s);
     }
-    if (t < 16) sum_h[t] = sum_o[t] = 0.f;
+    for (int i = 0; i < S + 2; ++i) fetch_scalars();
+    if (t < 32) sums[0][t] = sums[1][t] = 0.f;
 
-    const int col[2] = {t * 8, (t + nt) * 8};
-    const bool live[2] = {col[0] < p.n, col[1] < p.n};
-    Vec8<T> pre[2];
-    float2 coef[8];      // alpha * post [* gate]
+    int col[V];
+    bool live[V];
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-        Vec8<T> w, g;
-        w.zero(); g.zero(); pre[v].zero();
-        if (live[v]) {
-            w.load(p.post + col[v] * ES);
-            if (GATE == GATE_ROW) g.load(p.gate + col[v] * ES);
-            if (ES == 2) pre[v].load(p.pre + col[v] * ES);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            coef[4 * v + i] = mul2(w.get(i), splat2(p.alpha));
-            if (GATE == GATE_ROW) coef[4 * v + i] = mul2(coef[4 * v + i], g.get(i));
-        }
+    for (int v = 0; v < V; ++v) {
+        col[v] = (t + v * nt) * 8;
+        live[v] = col[v] < p.n;
     }
-    float2 a_pre[8], a_b[8], a_post[ROWS ? 8 : 1];
+    Vec8<T> pre[V];
+    float2 coef[4 * V];      // alpha * post [* gate]
+    auto coefficients = [&](int g) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        a_pre[i] = a_b[i] = make_float2(0.f, 0.f);
-        if (ROWS) a_post[i] = make_float2(0.f, 0.f);
-    }
-    __syncthreads();
-
-    // scales of the codes and 1/rms of a row, fetched one row ahead
-    struct RowScalars { float so[2], sh[2], rp, rh; };
-    auto scalars = [&](int64_t j) {
-        RowScalars q{};
-        if (j < end) {
-            const int64_t g = ROWS ? j / R : 0, row = ROWS ? g + (j - g * R) * G : j;
-            q.rp = p.r_post[row];
-            q.rh = p.r_pre[row];
-            if constexpr (CK != CODES_NONE) {
-#pragma unroll
-                for (int v = 0; v < 2; ++v)
-                    if (live[v]) {
-                        const int64_t at = row * (p.n >> 7) + (col[v] >> 7);
-                        q.so[v] = p.os_in[at];
-                        q.sh[v] = p.hs_in[at];
-                    }
+        for (int v = 0; v < V; ++v) {
+            Vec8<T> w, q;
+            w.zero(); q.zero();
+            if (live[v]) {
+                w.load(p.post + col[v] * ES);
+                if (GATE == GATE_ROW || GROUPS) q.load(p.gate + int64_t(g) * row_bytes + col[v] * ES);
             }
-        }
-        return q;
-    };
-    // this CTA's sum of the gradient of gate row g, whose positions are [g R, (g + 1) R)
-    auto flush_gate = [&](int64_t g) {
-        const bool whole = g * R >= begin && (g + 1) * R <= end;
-        float* slot = p.part + (int64_t(blockIdx.x) * PART_ROWS + (g * R < begin ? PART_HEAD : PART_TAIL)) * p.n;
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            float2 d[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                d[i] = mul2(a_b[4 * v + i], coef[4 * v + i]);
-                a_b[4 * v + i] = make_float2(0.f, 0.f);
-            }
-            if (live[v]) {
-                if (whole) {
-                    Vec8<T> w;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w.set(i, d[i]);
-                    w.store(p.dgate + g * row_bytes + col[v] * ES);
-                } else {
-                    float4* dst = reinterpret_cast<float4*>(slot + col[v]);
-                    dst[0] = make_float4(d[0].x, d[0].y, d[1].x, d[1].y);
-                    dst[1] = make_float4(d[2].x, d[2].y, d[3].x, d[3].y);
-                }
+                coef[4 * v + i] = mul2(w.get(i), splat2(p.alpha));
+                if (GATE == GATE_ROW || GROUPS) coef[4 * v + i] = mul2(coef[4 * v + i], q.get(i));
             }
         }
     };
-
-    bool dead = false;
-    int s = 0;
-    uint32_t phase = 0;
-    RowScalars next = scalars(begin);
-    int64_t g = ROWS ? begin / R : 0, g_end = (g + 1) * R;      // group of the row, position where it ends
-    for (int64_t j = begin; j < end; ++j) {
-        const RowScalars cur = next;
-        next = scalars(j + 1);
-        if (ROWS && j == g_end) { flush_gate(g); ++g; g_end += R; }
-        const int64_t row = ROWS ? g + (j - g * R) * G : j;
-        mbar_wait_or_mark<true>(&full[s], phase, DEVERR_FULL_WAIT, dead);
-        const uint8_t* st = ring + size_t(s) * stage_bytes;
-
-        auto values = [&](uint32_t off, int v, float scale, float2* e) {   // o or h
-            if constexpr (CK == CODES_NONE) {
-                Vec8<T> w;
-                w.load(st + off + col[v] * ES);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = w.get(i);
-            } else {
-                decode8<CK>(*reinterpret_cast<const uint2*>(st + off + col[v]), scale, e);
-            }
-        };
-        float2 acc = make_float2(0.f, 0.f);
+    for (int v = 0; v < V; ++v) {
+        pre[v].zero();
+        if (ES == 2 && live[v]) pre[v].load(p.pre + col[v] * ES);
+    }
+    At at2 = start(begin);         // row of pass 2
+    coefficients(at2.g);
+    float2 a_pre[4 * V], a_b[4 * V];
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
+    for (int i = 0; i < 4 * V; ++i) a_pre[i] = a_b[i] = make_float2(0.f, 0.f);
+    // dpost's sums of GATE_GROUPS, behind the ring, each thread's own
+    float4* a_post = reinterpret_cast<float4*>(ring + size_t(S) * stage_bytes) + t;
+    if constexpr (GROUPS)
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) a_post[i * nt] = make_float4(0.f, 0.f, 0.f, 0.f);
+
+    // What the elements of vector v are multiplied by to be hn (which 1) or on (0): 1/rms, times the scale of the codes' block.
+    auto factor = [&](const float* sc, int which, int v) {
+        const float r = sc[2 * nb + which];
+        return CK == CODES_NONE ? r : r * sc[(which ? nb : 0) + (col[v] >> 7)];
+    };
+    Kept<T, CK> ok[V];       // o of the row between passes 2 and 3
+    auto pass1 = [&](const uint8_t* st, const float* sc) {
+        float part = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
             if (live[v]) {
                 Vec8<T> dy, w;
-                float2 h[4];
+                Kept<T, CK> hk;
+                float2 h[4], acc = make_float2(0.f, 0.f);
                 dy.load(st + col[v] * ES);
-                values(off_h, v, cur.sh[v], h);
+                hk.load(st + off_h, col[v]);
+                hk.get(h);
                 if (ES == 2) w = pre[v]; else w.load(p.pre + col[v] * ES);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc = fma2(mul2(dy.get(i), w.get(i)), h[i], acc);
+                part = fmaf(acc.x + acc.y, factor(sc, 1, v), part);
             }
-        const float rh = cur.rh, rp = cur.rp;
-        const float ch = cta_sum(acc.x + acc.y, sum_h) * p.inv_n * rh * rh;      // mean(t * hn) * r_pre
-        acc = make_float2(0.f, 0.f);
-        float2 u[8];
+        return part;
+    };
+    auto pass2 = [&](const uint8_t* st, const float* sc, float ch, float2* u, uint8_t* dx_row) {   // ch: mean(t * hn)
+        const float rh = sc[2 * nb + 1];
+        float part = 0.f;
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
+        for (int v = 0; v < V; ++v)
             if (live[v]) {
-                Vec8<T> dy, din, w, gt, dx;
-                float2 h[4], o[4];
+                Vec8<T> dy, din, w, gt, dx, dg;
+                Kept<T, CK> hk;
+                float2 h[4], o[4], acc = make_float2(0.f, 0.f);
                 dy.load(st + col[v] * ES);
-                values(off_h, v, cur.sh[v], h);
-                values(off_o, v, cur.so[v], o);
+                hk.load(st + off_h, col[v]);
+                hk.get(h);
+                ok[v].load(st + off_o, col[v]);
+                ok[v].get(o);
                 if (has_dh) din.load(st + off_dh + col[v] * ES); else din.zero();
                 if (ES == 2) w = pre[v]; else w.load(p.pre + col[v] * ES);
-                if (ROWS) gt.load(st + off_g + col[v] * ES);
+                if (EACH) gt.load(st + off_g + col[v] * ES);
+                const float fh = factor(sc, 1, v), fo = factor(sc, 0, v);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 hn = mul2(h[i], splat2(rh)), gy = dy.get(i), on = mul2(o[i], splat2(rp));
-                    float2 d = fma2(hn, splat2(-ch), mul2(mul2(gy, w.get(i)), splat2(rh)));
-                    d = add2(d, din.get(i));
+                    const float2 hn = mul2(h[i], splat2(fh)), on = mul2(o[i], splat2(fo)), gy = dy.get(i);
+                    float2 d = fma2(fma2(hn, splat2(-ch), mul2(gy, w.get(i))), splat2(rh), din.get(i));
                     dx.set(i, d);
                     a_pre[4 * v + i] = fma2(gy, hn, a_pre[4 * v + i]);
-                    a_b[4 * v + i] = fma2(d, on, a_b[4 * v + i]);
-                    if constexpr (ROWS) {
+                    if constexpr (EACH) {
+                        dg.set(i, mul2(mul2(d, on), coef[4 * v + i]));
                         d = mul2(d, gt.get(i));
-                        a_post[4 * v + i] = fma2(d, on, a_post[4 * v + i]);
                     }
+                    a_b[4 * v + i] = fma2(d, on, a_b[4 * v + i]);
                     u[4 * v + i] = mul2(d, coef[4 * v + i]);
-                    acc = fma2(u[4 * v + i], o[i], acc);
+                    acc = fma2(u[4 * v + i], on, acc);
                 }
-                dx.store(p.dx + row * row_bytes + col[v] * ES);
+                dx.store(dx_row + col[v] * ES);
+                if (EACH) dg.store(p.dgate + (dx_row - p.dx) + col[v] * ES);
+                part += acc.x + acc.y;
             }
-        const float co = cta_sum(acc.x + acc.y, sum_o) * p.inv_n * rp * rp;      // mean(u * on) * r_post
+        if constexpr (GROUPS) {
+            // the last row of its group here: the group's gradient, its share of dpost, and B starts again
+            if (at2.left == 1 || at2.j + 1 == end) {
+                const int g0 = at2.g * R;
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
+                for (int v = 0; v < V; ++v)
+                    if (live[v]) {
+                        Vec8<T> w, q;
+                        w.load(p.post + col[v] * ES);
+                        q.load(p.gate + int64_t(at2.g) * row_bytes + col[v] * ES);
+                        float2 d[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) d[i] = mul2(mul2(w.get(i), splat2(p.alpha)), a_b[4 * v + i]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float4& sum = a_post[(2 * v + i) * nt];
+                            const float2 lo = mul2(a_b[4 * v + 2 * i], q.get(2 * i)), hi = mul2(a_b[4 * v + 2 * i + 1], q.get(2 * i + 1));
+                            sum = make_float4(sum.x + lo.x, sum.y + lo.y, sum.z + hi.x, sum.w + hi.y);
+                            a_b[4 * v + 2 * i] = a_b[4 * v + 2 * i + 1] = make_float2(0.f, 0.f);
+                        }
+                        if (g0 >= begin && g0 + R <= end) {
+                            Vec8<T> out;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) out.set(i, d[i]);
+                            out.store(p.dgate + int64_t(at2.g) * row_bytes + col[v] * ES);
+                        } else {
+                            float4* dst = reinterpret_cast<float4*>(p.part + (int64_t(blockIdx.x) * PART_ROWS + (g0 < begin ? PART_HEAD : PART_TAIL)) * p.n + col[v]);
+                            dst[0] = make_float4(d[0].x, d[0].y, d[1].x, d[1].y);
+                            dst[1] = make_float4(d[2].x, d[2].y, d[3].x, d[3].y);
+                        }
+                    }
+                if (at2.j + 1 < end) coefficients(at2.g + 1);
+            }
+        }
+        return part;
+    };
+    auto pass3 = [&](const float* sc, float co, const float2* u, uint8_t* row) {      // co: mean(u * on)
+        const float rp = sc[2 * nb];
+#pragma unroll
+        for (int v = 0; v < V; ++v)
             if (live[v]) {
                 Vec8<T> d;
                 float2 o[4];
-                values(off_o, v, cur.so[v], o);
+                ok[v].get(o);
+                const float c = -co * rp * factor(sc, 0, v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d.set(i, fma2(mul2(o[i], splat2(rp)), splat2(-co), mul2(u[4 * v + i], splat2(rp))));
-                d.store(p.dout + row * row_bytes + col[v] * ES);
+                for (int i = 0; i < 4; ++i) d.set(i, fma2(o[i], splat2(c), mul2(u[4 * v + i], splat2(rp))));
+                d.store(row + col[v] * ES);
             }
-        __syncthreads();      // every thread has read the stage
-        if (t == 0 && j + S < end) fetch(j + S, s);
-        if (++s == S) { s = 0; phase ^= 1u; }
+    };
+
+    bool dead = false;
+    float2 u[4 * V];
+    copies_wait<0>();
+    __syncthreads();
+    mbar_wait_or_mark<true>(&full[0], 0u, DEVERR_FULL_WAIT, dead);
+    uint8_t *dx_row = p.dx + int64_t(at2.row) * row_bytes, *do_row = p.dout + int64_t(at2.row) * row_bytes;
+    auto next_row = [&]() {
+        advance(at2);
+        if (GROUPS) {
+            dx_row = p.dx + int64_t(at2.row) * row_bytes;
+            do_row = p.dout + int64_t(at2.row) * row_bytes;
+        } else {
+            dx_row += row_bytes;
+            do_row += row_bytes;
+        }
+    };
+    if (S >= 2) {
+        int sl = 0, sc = 0, par = 0;                 // stage, slot of the scalars of the row of pass 2
+        uint32_t ph = 0;
+        const uint8_t* st = ring;
+        float2 sum = cta_sum2(pass1(st, scal[0]), 0.f, sums[par]);
+        par ^= 1;
+        float part2 = pass2(st, scal[0], sum.x * p.inv_n, u, dx_row);
+        while (true) {
+            const bool more = at2.j + 1 < end;
+            const int done = sl, sc3 = sc;
+            float part1 = 0.f;
+            if (more) {
+                if (++sl == S) { sl = 0; ph ^= 1u; }
+                if (++sc == DEPTH) sc = 0;
+                st = ring + size_t(sl) * stage_bytes;
+                mbar_wait_or_mark<true>(&full[sl], ph, DEVERR_FULL_WAIT, dead);
+                part1 = pass1(st, scal[sc]);
+            }
+            copies_wait<1>();
+            sum = cta_sum2(part1, part2, sums[par]);
+            par ^= 1;
+            // behind that barrier every thread has read the stage of the row whose pass 2 came before it
+            if (t == 0 && at2.j + S < end) fetch(done);
+            fetch_scalars();
+            pass3(scal[sc3], sum.y * p.inv_n, u, do_row);
+            if (!more) break;
+            next_row();
+            part2 = pass2(st, scal[sc], sum.x * p.inv_n, u, dx_row);
+        }
+    } else {
+        // one row fills the shared memory: float32 rows of more than about 7000 columns
+        int sc = 0;
+        uint32_t ph = 0;
+        while (true) {
+            float2 sum = cta_sum2(pass1(ring, scal[sc]), 0.f, sums[0]);
+            const float part = pass2(ring, scal[sc], sum.x * p.inv_n, u, dx_row);
+            fetch_scalars();
+            copies_wait<0>();
+            sum = cta_sum2(part, 0.f, sums[1]);
+            if (t == 0 && at2.j + 1 < end) fetch(0);
+            pass3(scal[sc], sum.x * p.inv_n, u, do_row);
+            if (at2.j + 1 == end) break;
+            next_row();
+            if (++sc == DEPTH) sc = 0;
+            ph ^= 1u;
+            mbar_wait_or_mark<true>(&full[0], ph, DEVERR_FULL_WAIT, dead);
+        }
     }
-    if (ROWS) flush_gate(g);      // begin < end: the grid has no more CTAs than there are rows
-    float* part = p.part + int64_t(blockIdx.x) * PART_ROWS * p.n;
+    grid_go();
+    copies_wait<0>();
+    float* out = p.part + int64_t(blockIdx.x) * PART_ROWS * p.n;
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
+    for (int v = 0; v < V; ++v)
         if (live[v]) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float2 *a = a_pre + 4 * v + 2 * i, *b = ROWS ? a_post + (ROWS ? 4 * v + 2 * i : 0) : a_b + 4 * v + 2 * i;
-                reinterpret_cast<float4*>(part + PART_PRE * p.n + col[v])[i] = make_float4(a[0].x, a[0].y, a[1].x, a[1].y);
-                reinterpret_cast<float4*>(part + PART_POST * p.n + col[v])[i] = make_float4(b[0].x, b[0].y, b[1].x, b[1].y);
+                const float2 *a = a_pre + 4 * v + 2 * i, *b = a_b + 4 * v + 2 * i;
+                reinterpret_cast<float4*>(out + PART_PRE * p.n + col[v])[i] = make_float4(a[0].x, a[0].y, a[1].x, a[1].y);
+                reinterpret_cast<float4*>(out + PART_POST * p.n + col[v])[i] = GROUPS ? a_post[(2 * v + i) * nt] : make_float4(b[0].x, b[0].y, b[1].x, b[1].y);
             }
         }
 }
@@ -415,55 +535,62 @@ __global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const Pair
 // The CTAs' sums, added in the order of the CTAs: blockIdx.y 0 dpre, 1 dpost (and the gradient of a gate of one row),
 // from 2 on the gate's groups that several CTAs share.
 template <typename T>
-__global__ void __launch_bounds__(1024) pair_reduce_kernel(const float* part, int ctas, int64_t M, int64_t G, int n, float alpha,
-                                                           const T* post, const T* gate, float* dpost, float* dpre, T* dgate) {
+__global__ void __launch_bounds__(256) pair_reduce_kernel(const float* part, int ctas, int M, int G, int n, float alpha, const T* post,
+                                                           const T* gate, float* dpost, float* dpre, T* dgate) {
     __shared__ float red[32][33];
-    const int c = threadIdx.x & 31, l = threadIdx.x >> 5;
-    const int col = blockIdx.x * 32 + c;             // n is a multiple of 128
-    const int64_t R = M / G;
+    grid_wait();                                     // for the kernel whose sums these are
+    const int c = (threadIdx.x & 7) * 4, l = threadIdx.x >> 3;       // four columns, every 32nd CTA's sums
+    const int R = M / G, q = M / ctas, rest = M % ctas;
+    auto first_of = [&](int b) { return b * q + min(b, rest); };                 // pair_first
+    auto owner = [&](int j) { return j < rest * (q + 1) ? j / (q + 1) : rest + (j - rest * (q + 1)) / q; };   // the CTA of a position
     // where there are fewer groups than borders between CTAs every group is looked at, else every border
-    const int64_t borders = ctas - 1, looks = G > 1 ? (G <= borders ? G : borders) : 0;
-    for (int64_t k = blockIdx.y; k < 2 + looks; k += gridDim.y) {
-        int64_t b0 = 0, b1 = ctas, g = 0;            // CTAs [b0, b1), their rows of scratch
-        int first = int(k), others = int(k);
+    const int borders = ctas - 1, looks = G > 1 && G < M ? min(G, borders) : 0;
+    for (int k = blockIdx.y; k < 2 + looks; k += gridDim.y) {
+        int b0 = 0, b1 = ctas, g = 0;                // CTAs [b0, b1), their rows of scratch
+        int first = k, others = k;
         if (k >= 2) {
             g = k - 2;
             if (G > borders) {
-                const int64_t at = pair_first(k - 1, ctas, M);        // where CTA k - 1 begins
+                const int at = first_of(k - 1);      // where CTA k - 1 begins
                 g = at / R;
-                if (at == g * R || pair_first(k - 2, ctas, M) > g * R) continue;   // between two groups, or not the group's first border
+                if (at == g * R || first_of(k - 2) > g * R) continue;   // between two groups, or not the group's first border
             }
-            b0 = g * R * ctas / M;
-            while (b0 > 0 && pair_first(b0, ctas, M) > g * R) --b0;
-            while (pair_first(b0 + 1, ctas, M) <= g * R) ++b0;
-            b1 = b0 + 1;
-            while (b1 < ctas && pair_first(b1, ctas, M) < (g + 1) * R) ++b1;
+            b0 = owner(g * R);
+            b1 = owner((g + 1) * R - 1) + 1;
             if (b1 == b0 + 1) continue;              // one CTA has the whole group and has written it
             first = PART_TAIL;
             others = PART_HEAD;
         }
-        float a = 0.f;
-        for (int64_t b = b0 + l; b < b1; b += 32) a += part[(b * PART_ROWS + (b == b0 ? first : others)) * n + col];
-        red[l][c] = a;
-        __syncthreads();
-        if (l == 0) {
-            float v = red[0][c];
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int b = b0 + l; b < b1; b += 8 * 32) {  // eight loads in flight; the order of the sum is that of the CTAs l, l + 32, ...
+            float4 v[8];
 #pragma unroll
-            for (int i = 1; i < 32; ++i) v += red[i][c];
+            for (int i = 0; i < 8; ++i) {
+                const int at = b + 32 * i;
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at < b1) v[i] = *reinterpret_cast<const float4*>(part + (int64_t(at) * PART_ROWS + (at == b0 ? first : others)) * n + blockIdx.x * 32 + c);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a = make_float4(a.x + v[i].x, a.y + v[i].y, a.z + v[i].z, a.w + v[i].w);
+        }
+        red[l][c] = a.x; red[l][c + 1] = a.y; red[l][c + 2] = a.z; red[l][c + 3] = a.w;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            const int col = blockIdx.x * 32 + threadIdx.x;          // n is a multiple of 128
+            float v = red[0][threadIdx.x];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) v += red[i][threadIdx.x];
             if (k == 0) {
                 dpre[col] = v;
             } else if (k == 1) {
-                if (G > 1) v *= alpha;
-                else {
-                    v *= alpha;
-                    if (gate) {
-                        dgate[col] = T(v * float(post[col]));
-                        v *= float(gate[col]);
-                    }
+                v *= alpha;
+                if (G == 1 && gate) {
+                    dgate[col] = T(v * float(post[col]));
+                    v *= float(gate[col]);
                 }
                 dpost[col] = v;
             } else {
-                dgate[g * n + col] = T(v);
+                dgate[int64_t(g) * n + col] = T(v);
             }
         }
         __syncthreads();
@@ -472,79 +599,89 @@ __global__ void __launch_bounds__(1024) pair_reduce_kernel(const float* part, in
 
 int pair_threads(int64_t n) { return int((n / 16 + 31) / 32 * 32); }
 
-// CTAs per SM and stages for rows of `bytes` per stage: `threads` in all on an SM, at least two stages
-void pair_shape(int threads_per_sm, int nt, int64_t bytes, int& per_sm, int& stages) {
+// CTAs per SM and stages of `bytes` each, with `fixed` bytes beside them: `threads` in all on an SM, at least two stages
+void pair_shape(int threads_per_sm, int nt, int64_t bytes, int64_t fixed, int& per_sm, int& stages) {
     per_sm = std::max(1, std::min(32, threads_per_sm / nt));
     while (true) {
-        stages = int(std::min<int64_t>(kPairMaxStages, (kPairSmem / per_sm - kPairSlack) / bytes));
+        stages = int(std::min<int64_t>(kPairMaxStages, (kPairSmem / per_sm - kPairSlack - fixed) / bytes));
         if (stages >= 2 || per_sm == 1) break;
         per_sm = (per_sm + 1) / 2;
     }
     stages = std::max(stages, 1);
 }
 
-constexpr int kPairBwdThreadsPerSm = 512;   // 128 registers a thread
+constexpr int kPairThreadsPerSm = 512;   // 128 registers a thread
 
 template <typename F>
 int pair_launch(F kern, int64_t grid, int nt, int64_t smem, const PairParams& p, const char* what, cudaStream_t stream) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return int(e); }
+    if (smem > 0) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return int(e); }
+    }
     kern<<<unsigned(grid), nt, size_t(smem), stream>>>(p);
     return check_launch(what);
 }
 
 template <typename T>
-int pair_fwd_typed(PairParams& p, int ck, cudaStream_t stream) {
-    const int nt = pair_threads(p.n);
-    const bool gated = p.gate && p.G > 1;
-    const int64_t bytes = int64_t(p.n) * sizeof(T) * (gated ? 3 : 2);
-    int per_sm;
-    pair_shape(1024 / (sizeof(T) == 2 ? 1 : 2), nt, bytes, per_sm, p.stages);
-    const int64_t grid = std::min<int64_t>(p.M, int64_t(sm_count()) * per_sm);
-    auto go = [&](auto kern) { return pair_launch(kern, grid, nt, bytes * p.stages, p, "pair_fwd_kernel", stream); };
-    if (ck == CODES_INT8) return gated ? go(pair_fwd_kernel<T, CODES_INT8, true>) : go(pair_fwd_kernel<T, CODES_INT8, false>);
-    if (ck == CODES_E4M3) return gated ? go(pair_fwd_kernel<T, CODES_E4M3, true>) : go(pair_fwd_kernel<T, CODES_E4M3, false>);
-    return gated ? go(pair_fwd_kernel<T, CODES_NONE, true>) : go(pair_fwd_kernel<T, CODES_NONE, false>);
+int pair_fwd_typed(const PairParams& p, int ck, cudaStream_t stream) {
+    auto go = [&](auto kern) { return pair_launch(kern, p.M, int((p.n * sizeof(T) / 32 + 31) / 32 * 32), 0, p, "pair_fwd_kernel", stream); };
+    if (ck == CODES_INT8) return go(pair_fwd_kernel<T, CODES_INT8>);
+    if (ck == CODES_E4M3) return go(pair_fwd_kernel<T, CODES_E4M3>);
+    return go(pair_fwd_kernel<T, CODES_NONE>);
 }
 
 int64_t pair_bwd_grid(int64_t M, int64_t n) {
-    return std::min<int64_t>(M, int64_t(sm_count()) * std::max(1, std::min(32, kPairBwdThreadsPerSm / pair_threads(n))));
+    return std::min<int64_t>(M, int64_t(sm_count()) * std::max(1, std::min(32, kPairThreadsPerSm / pair_threads(n))));
 }
 
 template <typename T>
 int pair_bwd_typed(PairParams& p, int ck, float* dpost, float* dpre, cudaStream_t stream) {
     const int nt = pair_threads(p.n);
     const int64_t code = ck == CODES_NONE ? int64_t(sizeof(T)) : 1;
-    const int64_t bytes = p.n * (int64_t(sizeof(T)) * (1 + (p.dh ? 1 : 0) + (p.gate && p.G > 1 ? 1 : 0)) + 2 * code);
+    const bool each = p.gate && p.G == p.M && p.M > 1, groups = p.gate && p.G > 1 && !each;
+    const int64_t bytes = p.n * (int64_t(sizeof(T)) * (1 + (p.dh ? 1 : 0) + (each ? 1 : 0)) + 2 * code);
     int per_sm;
-    pair_shape(kPairBwdThreadsPerSm, nt, bytes, per_sm, p.stages);
+    const int64_t fixed = groups ? int64_t(nt) * 64 : 0;
+    pair_shape(kPairThreadsPerSm, nt, bytes, fixed, per_sm, p.stages);
     const int64_t grid = std::min(pair_bwd_grid(p.M, p.n), int64_t(sm_count()) * per_sm);
-    auto go = [&](auto kern) { return pair_launch(kern, grid, nt, bytes * p.stages, p, "pair_bwd_kernel", stream); };
+    auto go = [&](auto kern) { return pair_launch(kern, grid, nt, bytes * p.stages + fixed, p, "pair_bwd_kernel", stream); };
     int rc;
     auto with = [&](auto codes) {
         constexpr int CK = decltype(codes)::value;
         if (!p.gate) return go(pair_bwd_kernel<T, CK, GATE_NONE>);
-        return p.G > 1 ? go(pair_bwd_kernel<T, CK, GATE_ROWS>) : go(pair_bwd_kernel<T, CK, GATE_ROW>);
+        if (p.G == 1) return go(pair_bwd_kernel<T, CK, GATE_ROW>);
+        return each ? go(pair_bwd_kernel<T, CK, GATE_EACH>) : go(pair_bwd_kernel<T, CK, GATE_GROUPS>);
     };
     if (ck == CODES_INT8) rc = with(std::integral_constant<int, CODES_INT8>{});
     else if (ck == CODES_E4M3) rc = with(std::integral_constant<int, CODES_E4M3>{});
     else rc = with(std::integral_constant<int, CODES_NONE>{});
     if (rc) return rc;
-    const int64_t looks = p.gate && p.G > 1 ? std::min<int64_t>(p.G, grid - 1) : 0;
-    pair_reduce_kernel<T><<<dim3(unsigned(p.n / 32), unsigned(2 + std::min<int64_t>(looks, 8))), 1024, 0, stream>>>(
-        p.part, int(grid), p.M, p.gate ? p.G : 1, p.n, p.alpha, reinterpret_cast<const T*>(p.post), reinterpret_cast<const T*>(p.gate),
-        dpost, dpre, reinterpret_cast<T*>(p.dgate));
-    return check_launch("pair_reduce_kernel");
+    const int64_t looks = groups ? std::min<int64_t>(p.G, grid - 1) : 0;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(p.n / 32), unsigned(2 + std::min<int64_t>(looks, 8)));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];      // it may be set up while the last CTAs above still run
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, pair_reduce_kernel<T>, static_cast<const float*>(p.part), int(grid), int(p.M), p.gate ? int(p.G) : 1,
+                                             p.n, p.alpha, reinterpret_cast<const T*>(p.post), reinterpret_cast<const T*>(p.gate), dpost, dpre,
+                                             reinterpret_cast<T*>(p.dgate));
+    if (e != cudaSuccess) { (void)cudaGetLastError(); set_error("pair_reduce_kernel: %s", cudaGetErrorString(e)); return int(e); }
+    return LH_OK;
 }
 
-bool unaligned(std::initializer_list<const void*> ps) {
+bool unaligned(std::initializer_list<const void*> ps, uintptr_t to = 16) {
     uintptr_t a = 0;
     for (const void* q : ps) a |= reinterpret_cast<uintptr_t>(q);
-    return (a & 15) != 0;
+    return (a & (to - 1)) != 0;
 }
 
 int pair_check(const char* what, int dtype, int64_t M, int64_t n, const void* gate, int64_t G, int codes) {
     if (dtype != LH_BF16 && dtype != LH_F16 && dtype != LH_F32) return fail_arg("%s: dtype must be bf16, f16 or f32", what);
+    if (M > 0x7fffffff) return fail_arg("%s: too many rows", what);
     if (M < 0 || n <= 0 || n > kPairMaxN || (n % 128) != 0)
         return fail_arg("%s: need n %% 128 == 0 and n <= %d (M=%lld n=%lld)", what, kPairMaxN, (long long)M, (long long)n);
     if (codes < CODES_NONE || codes > CODES_E4M3) return fail_arg("%s: codes must be 0 (none), 1 (int8) or 2 (e4m3)", what);
@@ -572,6 +709,7 @@ int pair_fwd(const void* x, const void* o, const void* post, const void* pre, co
     p.x = b(x); p.o = b(o); p.post = b(post); p.pre = b(pre); p.gate = b(gate);
     p.M = M; p.G = G; p.n = int(n); p.alpha = alpha; p.eps = eps; p.inv_n = 1.0f / float(n);
     p.h = static_cast<uint8_t*>(h); p.y = static_cast<uint8_t*>(y); p.r_post = r_post; p.r_pre = r_pre;
+    p.wide = !unaligned({x, o, h, y, post, pre, gate}, 32);
     p.oq = static_cast<uint8_t*>(oq); p.os = os; p.hq = static_cast<uint8_t*>(hq); p.hs = hs;
     if (dtype == LH_BF16) return pair_fwd_typed<__nv_bfloat16>(p, codes, stream);
     if (dtype == LH_F16) return pair_fwd_typed<__half>(p, codes, stream);

@@ -13,6 +13,9 @@ from linghe_b200 import _lib
 def int8_gemm(a, b, a_s, b_s, out_dtype=torch.bfloat16):
     """c [..., N] = (a @ b.T) * a_s[:, None] * b_s for int8 `a` [..., K] and `b` [N, K], float32 `a_s` (one per row of
     a) and `b_s` [N].  K is a multiple of 16, at most 131056; out_dtype bf16, fp16 or fp32."""
+    host = _lib.host()
+    if host is not None:   # the same steps in C++ (host/lh_host.cpp)
+        return host.int8_gemm(a, b, a_s, b_s, out_dtype)
     assert out_dtype in _lib._DTYPES, f"unsupported out_dtype {out_dtype}"
     N, K = b.shape
     assert a.dim() >= 1 and a.shape[-1] == K, f"a has {a.shape[-1]} columns, b has {K}"
@@ -32,6 +35,9 @@ def int8_linear(x, w, w_s, smooth_scale=None, out_dtype=None):
 
     `smooth_scale` (float32 [K]): x is divided by it before it is quantised; the weights hold the product with it.
     The result has `out_dtype`, that of x by default."""
+    host = _lib.host()
+    if host is not None:
+        return host.int8_linear(x, w, w_s, smooth_scale, out_dtype)
     if out_dtype is None:
         out_dtype = x.dtype
     assert out_dtype in _lib._DTYPES, f"unsupported out_dtype {out_dtype}"

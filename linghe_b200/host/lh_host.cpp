@@ -148,6 +148,243 @@ std::vector<at::Tensor> empty_many(const at::Tensor& ref, const std::vector<std:
 
 uintptr_t current_stream(int device) { return reinterpret_cast<uintptr_t>(c10::cuda::getCurrentCUDAStream(device).stream()); }
 
+// ---- the operators that keep activations in eight bits: the argument handling of utils/norm.py (rms_norm_pair_*),
+// utils/silu.py (silu_and_checkpoint_*), quant/token.py and gemm/int8_gemm.py, restated ----
+
+#define LH_NEED(cond, msg) \
+    do { if (!(cond)) raise_assert(msg); } while (0)
+
+// contiguous, on the device of `ref`, of `type` and `shape` (the checks of _lib.check_same)
+void check_same(const at::Tensor& ref, at::ScalarType type, const char* name, const at::Tensor& t) {
+    if (t.device() != ref.device()) raise_assert(std::string(name) + " is on " + t.device().str() + ", expected " + ref.device().str());
+    if (t.scalar_type() != type) raise_assert(std::string(name) + " is " + c10::toString(t.scalar_type()) + ", expected " + c10::toString(type));
+    if (!t.is_contiguous()) raise_assert(std::string(name) + " must be contiguous");
+}
+void check_same(const at::Tensor& ref, at::ScalarType type, const char* name, const at::Tensor& t, at::IntArrayRef shape) {
+    check_same(ref, type, name, t);
+    if (t.sizes() != shape) raise_assert(std::string(name) + " has another shape than expected");
+}
+
+const void* cptr(const OptT& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+float* fptr(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+const float* fptr(const OptT& t) { return t.has_value() ? static_cast<const float*>(t->data_ptr()) : nullptr; }
+
+int checkpoint_code(const std::optional<at::ScalarType>& type) {
+    if (!type.has_value()) return 0;
+    if (*type == at::kChar) return 1;
+    if (*type == at::kFloat8_e4m3fn) return 2;
+    raise_assert("checkpoint must be torch.int8 or torch.float8_e4m3fn");
+}
+
+int64_t rows_cols(const at::Tensor& x, int64_t& n) {
+    LH_NEED(x.dim() == 2 || x.dim() == 3, "x must be 2-D or 3-D");
+    n = x.size(-1);
+    return x.dim() == 3 ? x.size(0) * x.size(1) : x.size(0);
+}
+
+// rows of a gate whose shape is that of the last dimensions of x
+int64_t gate_rows(const OptT& gate, const at::Tensor& x) {
+    if (!gate.has_value()) return 0;
+    at::IntArrayRef shape = gate->sizes();
+    while (shape.size() > 1 && shape[0] == 1) shape = shape.slice(1);
+    LH_NEED(!shape.empty() && int64_t(shape.size()) <= x.dim() && shape == x.sizes().slice(x.dim() - shape.size()),
+            "gate must have the shape of the last dimensions of x");
+    int64_t g = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) g *= shape[i];
+    return g;
+}
+
+using Saved = std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>>;
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, Saved> rms_norm_pair_forward(
+    const at::Tensor& x, const at::Tensor& o, const at::Tensor& post, const at::Tensor& pre, const OptT& gate, double alpha, double eps,
+    const std::optional<at::ScalarType>& checkpoint) {
+    int64_t n = 0;
+    const int64_t M = rows_cols(x, n);
+    LH_NEED(n > 0 && n % 128 == 0 && n <= 8192, "need n % 128 == 0 and n <= 8192");
+    const int codes = checkpoint_code(checkpoint), dt = dtype_code(x);
+    check_device(x);
+    const at::ScalarType type = x.scalar_type();
+    check_same(x, type, "x", x);
+    check_same(x, type, "o", o, x.sizes());
+    check_same(x, type, "post_weight", post, {n});
+    check_same(x, type, "pre_weight", pre, {n});
+    if (gate.has_value()) check_same(x, type, "gate", *gate);
+    const int64_t G = gate_rows(gate, x);
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    const auto f32 = x.options().dtype(at::kFloat);
+    const at::Tensor h = at::empty(x.sizes(), x.options()), y = at::empty(x.sizes(), x.options()), rp = at::empty({M}, f32), rh = at::empty({M}, f32);
+    Saved saved;
+    at::Tensor oq, os, hq, hs;
+    if (codes) {
+        const auto q = x.options().dtype(*checkpoint);
+        oq = at::empty(x.sizes(), q); os = at::empty({M, n / 128}, f32);
+        hq = at::empty(x.sizes(), q); hs = at::empty({M, n / 128}, f32);
+        saved = std::make_tuple(oq, os, hq, hs);
+    }
+    check_rc(lh_rmsnorm_pair_fwd(x.data_ptr(), o.data_ptr(), post.data_ptr(), pre.data_ptr(), cptr(gate), dt, M, n, G, float(alpha), float(eps),
+                                 codes, h.data_ptr(), y.data_ptr(), fptr(rp), fptr(rh), codes ? oq.data_ptr() : nullptr, codes ? fptr(os) : nullptr,
+                                 codes ? hq.data_ptr() : nullptr, codes ? fptr(hs) : nullptr, c10::cuda::getCurrentCUDAStream().stream()),
+             "lh_rmsnorm_pair_fwd");
+    return {h, y, rp, rh, saved};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, OptT> rms_norm_pair_backward(
+    const at::Tensor& dy, const OptT& dh, const at::Tensor& o, const at::Tensor& h, const at::Tensor& post, const at::Tensor& pre,
+    const at::Tensor& rp, const at::Tensor& rh, const OptT& gate, double alpha, const OptT& os, const OptT& hs) {
+    int64_t n = 0;
+    const int64_t M = rows_cols(dy, n);
+    LH_NEED(n > 0 && n % 128 == 0 && n <= 8192, "need n % 128 == 0 and n <= 8192");
+    LH_NEED(os.has_value() == hs.has_value(), "o_scale and h_scale are given together");
+    const int codes = os.has_value() ? checkpoint_code(o.scalar_type()) : 0, dt = dtype_code(dy);
+    check_device(dy);
+    const at::ScalarType type = dy.scalar_type(), kept = codes ? o.scalar_type() : type;
+    check_same(dy, type, "grad_y", dy);
+    if (dh.has_value()) check_same(dy, type, "grad_h", *dh, dy.sizes());
+    check_same(dy, kept, "o", o, dy.sizes());
+    check_same(dy, kept, "h", h, dy.sizes());
+    if (codes) {
+        check_same(dy, at::kFloat, "o_scale", *os, {M, n / 128});
+        check_same(dy, at::kFloat, "h_scale", *hs, {M, n / 128});
+    }
+    check_same(dy, type, "post_weight", post, {n});
+    check_same(dy, type, "pre_weight", pre, {n});
+    check_same(dy, at::kFloat, "rms_post", rp, {M});
+    check_same(dy, at::kFloat, "rms_pre", rh, {M});
+    if (gate.has_value()) check_same(dy, type, "gate", *gate);
+    const int64_t G = gate_rows(gate, dy);
+    const c10::cuda::OptionalCUDAGuard guard(dy.device());
+    const auto f32 = dy.options().dtype(at::kFloat);
+    const int64_t nbytes = lh_scratch_bytes("rmsnorm_pair_bwd", M, n);
+    const at::Tensor dx = at::empty(dy.sizes(), dy.options()), dout = at::empty(dy.sizes(), dy.options()), dpost = at::empty({n}, f32),
+                     dpre = at::empty({n}, f32), scratch = at::empty({nbytes}, dy.options().dtype(at::kByte));
+    OptT dgate;
+    if (gate.has_value()) dgate = at::empty(gate->sizes(), dy.options());
+    check_rc(lh_rmsnorm_pair_bwd(dy.data_ptr(), cptr(dh), o.data_ptr(), fptr(os), h.data_ptr(), fptr(hs), post.data_ptr(), pre.data_ptr(),
+                                 cptr(gate), fptr(rp), fptr(rh), dt, M, n, G, float(alpha), codes, dx.data_ptr(), dout.data_ptr(), fptr(dpost),
+                                 fptr(dpre), ptr(dgate), scratch.data_ptr(), nbytes, c10::cuda::getCurrentCUDAStream().stream()),
+             "lh_rmsnorm_pair_bwd");
+    return {dx, dout, dpost, dpre, dgate};
+}
+
+int weight_code(const at::Tensor& ref, const OptT& w, int64_t M) {
+    if (!w.has_value()) return LH_F32;
+    check_same(ref, w->scalar_type(), "weight", *w, {M});
+    return dtype_code(*w);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> silu_and_checkpoint_forward(const at::Tensor& x, const OptT& w,
+                                                                           const std::optional<at::ScalarType>& checkpoint) {
+    LH_NEED(x.dim() == 2, "x must be 2-D");
+    const int64_t M = x.size(0), N = x.size(1);
+    LH_NEED(N > 0 && N % 256 == 0, "need N % 256 == 0");
+    const int codes = checkpoint_code(checkpoint), dt = dtype_code(x);
+    LH_NEED(codes != 0, "checkpoint must be torch.int8 or torch.float8_e4m3fn");
+    check_device(x);
+    check_same(x, x.scalar_type(), "x", x);
+    const int wt = weight_code(x, w, M);
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    const at::Tensor y = at::empty({M, N / 2}, x.options()), q = at::empty({M, N}, x.options().dtype(*checkpoint)),
+                     s = at::empty({M, N / 128}, x.options().dtype(at::kFloat));
+    check_rc(lh_silu_checkpoint_fwd(x.data_ptr(), cptr(w), dt, wt, codes, M, N / 2, y.data_ptr(), q.data_ptr(), fptr(s),
+                                    c10::cuda::getCurrentCUDAStream().stream()),
+             "lh_silu_checkpoint_fwd");
+    return {y, q, s};
+}
+
+std::tuple<at::Tensor, OptT> silu_and_checkpoint_backward(const at::Tensor& g, const at::Tensor& q, const at::Tensor& s, const OptT& w) {
+    LH_NEED(q.dim() == 2, "x_q must be 2-D");
+    const int64_t M = q.size(0), N = q.size(1);
+    LH_NEED(N > 0 && N % 256 == 0, "need N % 256 == 0");
+    const int codes = checkpoint_code(q.scalar_type()), dt = dtype_code(g);
+    check_device(g);
+    check_same(g, g.scalar_type(), "g", g, {M, N / 2});
+    check_same(g, q.scalar_type(), "x_q", q);
+    check_same(g, at::kFloat, "x_scale", s, {M, N / 128});
+    const int wt = weight_code(g, w, M);
+    const c10::cuda::OptionalCUDAGuard guard(g.device());
+    const at::Tensor dx = at::empty({M, N}, g.options());
+    OptT dw;
+    if (w.has_value()) dw = at::empty({M}, w->options());
+    check_rc(lh_silu_checkpoint_bwd(g.data_ptr(), q.data_ptr(), fptr(s), cptr(w), dt, wt, codes, M, N / 2, dx.data_ptr(), ptr(dw),
+                                    c10::cuda::getCurrentCUDAStream().stream()),
+             "lh_silu_checkpoint_bwd");
+    return {dx, dw};
+}
+
+// sizes [..., K] -> [..., N]
+std::vector<int64_t> last_dim(const at::Tensor& t, int64_t n) {
+    std::vector<int64_t> v = t.sizes().vec();
+    v.back() = n;
+    return v;
+}
+
+std::tuple<at::Tensor, at::Tensor> token_quant_int8(const at::Tensor& x, const OptT& smooth, OptT out, OptT scale) {
+    LH_NEED(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 16 == 0, "K must be a positive multiple of 16");
+    const int64_t K = x.size(-1), M = x.numel() / K;
+    const int dt = dtype_code(x);
+    check_device(x);
+    check_same(x, x.scalar_type(), "x", x);
+    if (smooth.has_value()) check_same(x, at::kFloat, "smooth_scale", *smooth, {K});
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    if (!out.has_value()) out = at::empty(x.sizes(), x.options().dtype(at::kChar));
+    if (!scale.has_value()) scale = at::empty({M}, x.options().dtype(at::kFloat));
+    check_same(x, at::kChar, "out", *out, x.sizes());
+    check_same(x, at::kFloat, "scale", *scale, {M});
+    check_rc(lh_token_quant_int8(x.data_ptr(), fptr(smooth), dt, M, K, out->data_ptr(), fptr(*scale), c10::cuda::getCurrentCUDAStream().stream()),
+             "lh_token_quant_int8");
+    return {*out, *scale};
+}
+
+int out_code(at::ScalarType t) {
+    switch (t) {
+        case at::kBFloat16: return LH_BF16;
+        case at::kHalf: return LH_F16;
+        case at::kFloat: return LH_F32;
+        default: raise_assert("unsupported out_dtype");
+    }
+}
+
+at::Tensor int8_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_s, const at::Tensor& b_s, at::ScalarType out_dtype) {
+    const int od = out_code(out_dtype);
+    LH_NEED(b.dim() == 2 && a.dim() >= 1 && a.size(-1) == b.size(1), "a and b must have the same number of columns");
+    const int64_t N = b.size(0), K = b.size(1);
+    LH_NEED(K > 0 && K % 16 == 0, "K must be a positive multiple of 16");
+    const int64_t M = a.numel() / K;
+    check_device(a);
+    check_same(a, at::kChar, "a", a);
+    check_same(a, at::kChar, "b", b);
+    check_same(a, at::kFloat, "a_s", a_s, {M});
+    check_same(a, at::kFloat, "b_s", b_s, {N});
+    const c10::cuda::OptionalCUDAGuard guard(a.device());
+    const at::Tensor c = at::empty(last_dim(a, N), a.options().dtype(out_dtype));
+    check_rc(lh_int8_gemm(a.data_ptr(), b.data_ptr(), fptr(a_s), fptr(b_s), c.data_ptr(), M, N, K, od, c10::cuda::getCurrentCUDAStream().stream()),
+             "lh_int8_gemm");
+    return c;
+}
+
+at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_s, const OptT& smooth, const std::optional<at::ScalarType>& out_dtype) {
+    const at::ScalarType type = out_dtype.has_value() ? *out_dtype : x.scalar_type();
+    const int od = out_code(type), dt = dtype_code(x);
+    LH_NEED(w.dim() == 2 && x.dim() >= 1 && x.size(-1) == w.size(1), "x and w must have the same number of columns");
+    const int64_t N = w.size(0), K = w.size(1);
+    LH_NEED(K > 0 && K % 16 == 0, "K must be a positive multiple of 16");
+    const int64_t M = x.numel() / K;
+    check_device(x);
+    check_same(x, x.scalar_type(), "x", x);
+    check_same(x, at::kChar, "w", w);
+    check_same(x, at::kFloat, "w_s", w_s, {N});
+    if (smooth.has_value()) check_same(x, at::kFloat, "smooth_scale", *smooth, {K});
+    const c10::cuda::OptionalCUDAGuard guard(x.device());
+    const at::Tensor c = at::empty(last_dim(x, N), x.options().dtype(type));
+    const at::Tensor ws = at::empty({M * K + 4 * M}, x.options().dtype(at::kByte));      // codes, then scales: K is a multiple of 16
+    uint8_t* q = static_cast<uint8_t*>(ws.data_ptr());
+    check_rc(lh_int8_linear(x.data_ptr(), fptr(smooth), dt, w.data_ptr(), fptr(w_s), q, reinterpret_cast<float*>(q + M * K), c.data_ptr(), M, N, K,
+                            od, c10::cuda::getCurrentCUDAStream().stream()),
+             "lh_int8_linear");
+    return c;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_lh_host, m) {
@@ -157,4 +394,11 @@ PYBIND11_MODULE(_lh_host, m) {
 #include "lh_host_bindings.inc"
     m.def("rms_norm_and_block_quant_forward", &rms_norm_and_block_quant_forward);
     m.def("silu_and_block_quant_forward", &silu_and_block_quant_forward);
+    m.def("rms_norm_pair_forward", &rms_norm_pair_forward);
+    m.def("rms_norm_pair_backward", &rms_norm_pair_backward);
+    m.def("silu_and_checkpoint_forward", &silu_and_checkpoint_forward);
+    m.def("silu_and_checkpoint_backward", &silu_and_checkpoint_backward);
+    m.def("token_quant_int8", &token_quant_int8);
+    m.def("int8_gemm", &int8_gemm);
+    m.def("int8_linear", &int8_linear);
 }

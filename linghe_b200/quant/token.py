@@ -14,6 +14,9 @@ def token_quant_int8(x, smooth_scale=None, out=None, scale=None):
     quantisers of this package.  scale = max(amax / 127, 1e-30), code = nearest(x / scale), ties to even; a row
     with a NaN or an infinity gets a NaN scale.  Weights [N, K] take the same call: one scale per output channel.
     Returns (out int8 like x, scale float32 [rows])."""
+    host = _lib.host()
+    if host is not None:   # the same steps in C++ (host/lh_host.cpp)
+        return host.token_quant_int8(x, smooth_scale, out, scale)
     K = x.shape[-1]
     assert x.dim() >= 1 and K > 0 and K % 16 == 0
     rows = x.numel() // K

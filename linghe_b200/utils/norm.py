@@ -224,6 +224,9 @@ def rms_norm_pair_forward(x, o, post_weight, pre_weight, gate=None, residual_sca
     rms_norm_pair_backward takes in their place.
     Returns (h like x, y like x, rms_post f32 [M], rms_pre f32 [M], saved): the rms are 1/rms per row of o and of h;
     saved is None or (o_q [.., n], o_scale f32 [M, n/128], h_q, h_scale).  Upstream has no such operator."""
+    host = _lib.host()
+    if host is not None:   # the same steps in C++ (host/lh_host.cpp)
+        return host.rms_norm_pair_forward(x, o, post_weight, pre_weight, gate, float(residual_scale), float(eps), checkpoint)
     M, n = _rows_cols(x)
     assert n > 0 and n % 128 == 0 and n <= 8192
     codes = _lib.checkpoint_code(checkpoint)
@@ -251,6 +254,10 @@ def rms_norm_pair_backward(grad_y, grad_h, o, h, post_weight, pre_weight, rms_po
     of the next block) may be None.  o and h are the forward pass's tensors, or with o_scale and h_scale their 8-bit
     checkpoints (`saved` of the forward pass; the outputs of triton_group_quant are a checkpoint too).
     Returns (dx, do like grad_y, dpost f32 [n], dpre f32 [n], dgate like gate or None)."""
+    host = _lib.host()
+    if host is not None:
+        return host.rms_norm_pair_backward(grad_y, grad_h, o, h, post_weight, pre_weight, rms_post, rms_pre, gate, float(residual_scale),
+                                           o_scale, h_scale)
     M, n = _rows_cols(grad_y)
     assert n > 0 and n % 128 == 0 and n <= 8192
     dt = grad_y.dtype

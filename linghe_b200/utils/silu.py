@@ -301,6 +301,9 @@ def silu_and_checkpoint_forward(x, weight=None, checkpoint=torch.int8):
     takes in its place: int8 or e4m3 codes with one float32 scale per 1x128 block.  `weight`: float32 or bf16 [M], one
     value per row (a routing weight).  n % 128 == 0.  Upstream has no such operator: its SwiGLU saves x.
     Returns (y [M, n] x.dtype, x_q [M, 2n], x_scale f32 [M, 2n/128])."""
+    host = _lib.host()
+    if host is not None:   # the same steps in C++ (host/lh_host.cpp)
+        return host.silu_and_checkpoint_forward(x, weight, checkpoint)
     M, N = x.shape
     assert N > 0 and N % 256 == 0
     codes = _lib.checkpoint_code(checkpoint)
@@ -318,6 +321,9 @@ def silu_and_checkpoint_forward(x, weight=None, checkpoint=torch.int8):
 def silu_and_checkpoint_backward(g, x_q, x_scale, weight=None):
     """Gradient of silu_and_checkpoint_forward from the checkpoint of x: g [M, n] -> (dx [M, 2n] g.dtype, dw like
     weight or None).  Any row-major 1x128 codes of x will do, triton_group_quant's among them."""
+    host = _lib.host()
+    if host is not None:
+        return host.silu_and_checkpoint_backward(g, x_q, x_scale, weight)
     M, N = x_q.shape
     assert N > 0 and N % 256 == 0
     codes = _lib.checkpoint_code(x_q.dtype)
