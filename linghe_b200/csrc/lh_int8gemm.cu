@@ -10,6 +10,7 @@
 #include "lh_umma.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -114,7 +115,8 @@ struct Int8Params {
     int64_t M;
     int N, K;
     int out_dtype;
-    int wide;            // a row of c starts on a 32-byte boundary
+    int wide;            // N is a multiple of 4 and the scales of b are aligned: four columns at a time
+    int mapped;          // c has a tensor map
 };
 
 __device__ __forceinline__ void store_one(const Int8Params& p, int64_t at, float v) {
@@ -123,41 +125,70 @@ __device__ __forceinline__ void store_one(const Int8Params& p, int64_t at, float
     else reinterpret_cast<__half*>(p.c)[at] = __float2half_rn(v);
 }
 
-// NC (a multiple of 16) sums of one row from column col on, scaled, rounded and stored
-template <int NC>
-__device__ __forceinline__ void store_row(const Int8Params& p, int64_t row, int col, const uint32_t* v, float sa) {
-    if (row >= p.M || col >= p.N) return;
-    const int64_t at = row * p.N + col;
-    if (p.wide && col + NC <= p.N) {
+// What an epilogue warp keeps in shared memory: the scales of its columns, fetched while the sums are not there yet, and
+// 32 rows x 128 bytes in which a piece of the result is turned from one row per lane to whole 128-byte lines.  One row per
+// lane straight to global memory is 32 lines per instruction: the store of a 256 x 256 tile took longer than 1024 of k.
+struct alignas(1024) EpiWarp {
+    static constexpr int COLS = 128, LD = 17;
+    uint8_t buf[32 * 128];
+    float sb[COLS];
+};
+
+// rows of c that no tensor map can describe (not a multiple of 16 bytes long): 32 rows (lane = row) x 16 columns through
+// shared memory, then 16 neighbouring lanes per row, element by element
+__device__ __forceinline__ void store_ragged(const Int8Params& p, int64_t row0, int col, const uint32_t* v, float sa, EpiWarp& w, const float* sb) {
+    const int lane = threadIdx.x & 31;
+    if (col >= p.N) return;
+    float* turn = reinterpret_cast<float*>(w.buf);
 #pragma unroll
-        for (int h = 0; h < NC; h += 16) {
-            float f[16];
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 sb = *reinterpret_cast<const float4*>(p.b_s + col + h + i);
-                f[i] = __int2float_rn(int(v[h + i])) * sa * sb.x;
-                f[i + 1] = __int2float_rn(int(v[h + i + 1])) * sa * sb.y;
-                f[i + 2] = __int2float_rn(int(v[h + i + 2])) * sa * sb.z;
-                f[i + 3] = __int2float_rn(int(v[h + i + 3])) * sa * sb.w;
-            }
-            if (p.out_dtype == LH_F32) {
-                uint8_t* dst = p.c + (at + h) * 4;
-#pragma unroll
-                for (int j = 0; j < 16; j += 8)
-                    st_global_256(dst + 4 * j, make_uint4(__float_as_uint(f[j]), __float_as_uint(f[j + 1]), __float_as_uint(f[j + 2]), __float_as_uint(f[j + 3])),
-                                  make_uint4(__float_as_uint(f[j + 4]), __float_as_uint(f[j + 5]), __float_as_uint(f[j + 6]), __float_as_uint(f[j + 7])));
-            } else {
-                uint32_t w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = p.out_dtype == LH_BF16 ? pack_bf16x2(f[2 * j], f[2 * j + 1]) : pack_f16x2(f[2 * j], f[2 * j + 1]);
-                st_global_256(p.c + (at + h) * 2, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]));
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (col + i < p.N) store_one(p, at + i, __int2float_rn(int(v[i])) * sa * p.b_s[col + i]);
+    for (int i = 0; i < 16; ++i) turn[lane * EpiWarp::LD + i] = __int2float_rn(int(v[i])) * sa * sb[i];
+    __syncwarp();
+    const int c = col + (lane & 15);
+#pragma unroll 4
+    for (int r = 0; r < 32; r += 2) {
+        const int64_t row = row0 + r + (lane >> 4);
+        if (row < p.M && c < p.N) store_one(p, row * p.N + c, turn[(r + (lane >> 4)) * EpiWarp::LD + (lane & 15)]);
     }
+    __syncwarp();
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src_smem, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x),
+                 "r"(y), "r"(smem_u32(src_smem))
+                 : "memory");
+}
+
+// 32 rows (lane = row) x 32 columns, scaled and rounded, into bytes [64 half, 64 half + 64) of the rows of the buffer (16-bit
+// types) or all 128 (float32), laid out with the 128-byte swizzle: 16-byte piece i of row r lies at piece i ^ (r & 7)
+__device__ __forceinline__ void turn_piece(const Int8Params& p, const uint32_t* v, float sa, EpiWarp& w, const float* sb, int half) {
+    const int lane = threadIdx.x & 31;
+    uint8_t* row = w.buf + lane * 128;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+        const float4 s0 = *reinterpret_cast<const float4*>(sb + i), s1 = *reinterpret_cast<const float4*>(sb + i + 4);
+        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __int2float_rn(int(v[i + j])) * sa * s[j];
+        if (p.out_dtype == LH_F32) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 4)
+                *reinterpret_cast<float4*>(row + ((((i + j) >> 2) ^ (lane & 7)) << 4)) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+        } else {
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = p.out_dtype == LH_BF16 ? pack_bf16x2(f[2 * j], f[2 * j + 1]) : pack_f16x2(f[2 * j], f[2 * j + 1]);
+            *reinterpret_cast<uint4*>(row + (((4 * half + (i >> 3)) ^ (lane & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+}
+
+// scales of COLS columns from n0 on into shared memory, 0 past the last
+__device__ __forceinline__ void fetch_scales(const Int8Params& p, int n0, int cols, float* sb) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    for (int i = lane; i < cols; i += 32) sb[i] = n0 + i < p.N ? p.b_s[n0 + i] : 0.f;
+    __syncwarp();
 }
 
 // Few tokens: the weights are read once and there is next to no arithmetic, so what counts is to have all of
@@ -259,12 +290,45 @@ __device__ __forceinline__ void tmem_ld_row32(uint32_t taddr, uint32_t (&v)[32])
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint32_t tmem_alloc(uint32_t* slot, uint32_t cols) {
+// NC (a multiple of 64) columns of 32 rows from tensor memory to c; read() is called when all of them are in registers
+template <int NC, typename F>
+__device__ __forceinline__ void store_sums(const Int8Params& p, const CUtensorMap* map_c, uint32_t taddr, int64_t row0, int n0, float sa, EpiWarp& w, F read) {
+    const int lane = threadIdx.x & 31;
+    const bool f32 = p.out_dtype == LH_F32;
+    uint32_t v[2][32];
+    tmem_ld_row32(taddr, v[0]);
+#pragma unroll
+    for (int c = 0; c < NC; c += 32) {
+        const uint32_t* u = v[(c / 32) & 1];
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (c + 32 < NC) tmem_ld_row32(taddr + c + 32, v[(c / 32 + 1) & 1]);      // the next piece on its way while this one is stored
+        else read();
+        if (!p.mapped) {
+            store_ragged(p, row0, n0 + c, u, sa, w, w.sb + c);
+            store_ragged(p, row0, n0 + c + 16, u + 16, sa, w, w.sb + c + 16);
+            continue;
+        }
+        const bool first = f32 || (c & 32) == 0;
+        if (first) {                              // the copy before has read the buffer
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+        }
+        turn_piece(p, u, sa, w, w.sb + c, (c >> 5) & 1);
+        if (f32 || (c & 32) != 0) {
+            fence_async_smem();
+            __syncwarp();
+            const int x = n0 + (f32 ? c : c - 32);
+            if (lane == 0) {
+                if (row0 < p.M && x < p.N) tma_store_2d(map_c, w.buf, x, int(row0));
+                bulk_commit();
+            }
+        }
+    }
+}
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    return 0;
 }
 __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
@@ -275,17 +339,19 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
 template <int TN>
 struct BigTile {
     static constexpr int STAGE = I_ATILE + TN * IKB;
-    static constexpr int STAGES = TN == 256 ? 4 : 6;
-    static constexpr int BAR_OFF = STAGES * STAGE;
-    static constexpr int SMEM = 1024 + BAR_OFF + 256;
+    static constexpr int STAGES = 5;
     static constexpr int EPI_WARPS = 8;
+    static constexpr int EPI_OFF = STAGES * STAGE;
+    static constexpr int BAR_OFF = EPI_OFF + EPI_WARPS * int(sizeof(EpiWarp));
+    static constexpr int SMEM = 1024 + BAR_OFF + 256;
     static constexpr int THREADS = 32 * (2 + EPI_WARPS);
     static_assert(SMEM <= 232448, "shared memory");
 };
 
 template <int TN>
 __global__ void __launch_bounds__(BigTile<TN>::THREADS, 1)
-int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Int8Params p) {
+int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Int8Params p) {
     using C = BigTile<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -356,45 +422,47 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
+        EpiWarp& epi = reinterpret_cast<EpiWarp*>(smem + C::EPI_OFF)[warp - 2];
         uint32_t n = 0;
         bool ok = true;
         for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
-            const int64_t row = tile / tiles_n * IM + quarter * 32 + lane;
+            const int64_t row0 = tile / tiles_n * IM + quarter * 32;
             const int n0 = int(tile % tiles_n) * TN + half * (TN / 2);
             const uint32_t buf = n & 1u;
-            const float sa = row < p.M ? p.a_s[row] : 0.f;
+            const float sa = row0 + lane < p.M ? p.a_s[row0 + lane] : 0.f;
+            fetch_scales(p, n0, TN / 2, epi.sb);
             ok = __all_sync(0xffffffffu, mbar_wait_inline(&acc_full[buf], (n >> 1) & 1u, DEVERR_PART_WAIT));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t base = tmem + (uint32_t(quarter * 32) << 16) + buf * TN + half * (TN / 2);
-#pragma unroll
-            for (int c = 0; c < TN / 2; c += 32) {
-                uint32_t v[32];
-                tmem_ld_row32(base + c, v);
-                if (c == TN / 2 - 32) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&acc_empty[buf]);
-                }
-                store_row<32>(p, row, n0 + c, v, sa);
-            }
+            store_sums<TN / 2>(p, &map_c, tmem + (uint32_t(quarter * 32) << 16) + buf * TN + half * (TN / 2), row0, n0, sa, epi, [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            });
         }
+        if (lane == 0) bulk_wait_all();
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_free(tmem, 2 * TN);
 }
 
-// Products of few tiles: a cluster of S CTAs shares k of one tile, adds the partial sums through distributed
-// shared memory and stores a share of the rows each.  The cluster's rank is the part of k.
-template <int TN>
-struct SplitTile {
-    static constexpr int STAGE = I_ATILE + TN * IKB;
-    static constexpr int STAGES = TN == 256 ? 4 : TN == 128 ? 6 : 8;
-    static constexpr int BAR_OFF = STAGES * STAGE;
+// The largest products: two CTAs of a cluster (a pair of SMs) share a 256 x 256 tile, tcgen05.mma.cta_group::2.  Each
+// brings in its 128 rows of a and its 128 rows of b, half of what the pair multiplies, so an SM takes 32 KB per 128 bytes of k
+// where the 128 x 256 tile above takes 48: that kernel waits for L2 (96 bytes per cycle and SM at the full rate of the tensor
+// cores), this one needs 64.  The leader (rank 0) issues for both; full[] counts in the leader's shared memory what both
+// bring, commits arrive in both CTAs, both read their half of the sums.
+struct PairTile {
+    static constexpr int TN = 256, TM = 256;
+    static constexpr int STAGE = 2 * I_ATILE;         // a: 16 KB, b: 16 KB
+    static constexpr int STAGES = 5;
+    static constexpr int EPI_WARPS = 8;
+    static constexpr int EPI_OFF = STAGES * STAGE;
+    static constexpr int BAR_OFF = EPI_OFF + EPI_WARPS * int(sizeof(EpiWarp));
     static constexpr int SMEM = 1024 + BAR_OFF + 256;
-    static constexpr int THREADS = 192;
-    static_assert(SMEM <= 232448 && IM * TN * 4 <= BAR_OFF, "shared memory");
+    static constexpr int THREADS = 32 * (2 + EPI_WARPS);
+    static_assert(SMEM <= 232448, "shared memory");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -405,21 +473,200 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint4 ld_cluster(uint32_t addr, uint32_t rank) {
-    uint4 v;
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void umma2_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .b32 r;\n\t"
-        "mapa.shared::cluster.u32 r, %4, %5;\n\t"
-        "ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [r];\n\t}"
-        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-        : "r"(addr), "r"(rank)
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
-    return v;
+}
+// arrives on the barrier of this offset in both CTAs when the MMAs issued so far are complete
+__device__ __forceinline__ void umma2_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"(uint16_t(3))
+                 : "memory");
+}
+// a tile into this CTA's shared memory, its bytes counted on a barrier of the pair
+__device__ __forceinline__ void tma2_load_2d(void* dst_smem, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst_smem)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// bounded wait for arrivals from both CTAs
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int code) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < (1u << 22); ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    atomicCAS(&g_device_status, 0, code);
+    return false;
+}
+
+// Tiles in the order of row bands of 8 tiles, down a column of a band before the next column: the tiles in flight then
+// share as few rows of a and of b as can be, and both stay in L2 where one of them alone would not.
+__device__ __forceinline__ void band_tile(int64_t tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+    constexpr int BAND = 8;
+    const int64_t per_band = int64_t(BAND) * tiles_n;
+    const int band = int(tile / per_band), rest = int(tile - band * per_band);
+    const int rows = min(BAND, tiles_m - band * BAND);
+    tn = rest / rows;
+    tm = band * BAND + (rest - tn * rows);
+}
+
+__global__ void __launch_bounds__(PairTile::THREADS, 1)
+int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Int8Params p) {
+    using C = PairTile;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);   // used in the leader
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* acc_full = empty + C::STAGES;
+    uint64_t* acc_empty = acc_full + 2;                                // used in the leader
+    uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const uint32_t rank = cluster_rank();
+    const int kblocks = (p.K + IKB - 1) / IKB, tiles_n = (p.N + C::TN - 1) / C::TN, tiles_m = int((p.M + C::TM - 1) / C::TM);
+    const int64_t tiles = int64_t(tiles_m) * tiles_n;
+    const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    if (t == 0) {
+        for (int i = 0; i < C::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * C::EPI_WARPS); }
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                              // the other CTA's barriers are set up, too
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(slot);
+    grid_wait();
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t ph = 0;
+        bool fresh = true, ok = true;
+        for (int64_t tile = first; tile < tiles && ok; tile += step) {
+            int tm, tn;
+            band_tile(tile, tiles_m, tiles_n, tm, tn);
+            const int m0 = tm * C::TM + int(rank) * IM, n0 = tn * C::TN + int(rank) * 128;
+            for (int kb = 0; kb < kblocks; ++kb) {
+                if (!fresh) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_inline(&empty[s], ph ^ 1u, DEVERR_EMPTY_WAIT));
+                    if (!ok) break;
+                }
+                if (elect_one()) {
+                    uint8_t* st = smem + size_t(s) * C::STAGE;
+                    const uint32_t bar = mapa(smem_u32(&full[s]), 0);
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * C::STAGE);
+                    tma2_load_2d(st, &map_a, kb * IKB, m0, bar);
+                    tma2_load_2d(st + I_ATILE, &map_b, kb * IKB, n0, bar);
+                }
+                if (++s == C::STAGES) { s = 0; ph ^= 1u; fresh = false; }
+            }
+        }
+    } else if (warp == 1) {
+        int s = 0;
+        uint32_t ph = 0, n = 0;
+        bool ok = rank == 0;
+        for (int64_t tile = first; tile < tiles && ok; tile += step, ++n) {
+            const uint32_t buf = n & 1u;
+            if (n >= 2) ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[buf], ((n >> 1) & 1u) ^ 1u, DEVERR_PART_WAIT));
+            for (int kb = 0; kb < kblocks && ok; ++kb) {
+                ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full[s], ph, DEVERR_FULL_WAIT));
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a = smem_u32(smem + size_t(s) * C::STAGE);
+                    const uint64_t da = umma_desc(a), db = umma_desc(a + I_ATILE);
+#pragma unroll
+                    for (int k4 = 0; k4 < IKB / 32; ++k4)
+                        umma2_i8(tmem + buf * C::TN, da + 2 * k4, db + 2 * k4, i8_idesc(C::TM, C::TN), (kb | k4) != 0);
+                    umma2_commit(&empty[s]);
+                    if (kb == kblocks - 1) umma2_commit(&acc_full[buf]);
+                }
+                if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        EpiWarp& epi = reinterpret_cast<EpiWarp*>(smem + C::EPI_OFF)[warp - 2];
+        uint32_t n = 0;
+        bool ok = true;
+        for (int64_t tile = first; tile < tiles && ok; tile += step, ++n) {
+            int tm, tn;
+            band_tile(tile, tiles_m, tiles_n, tm, tn);
+            const int64_t row0 = int64_t(tm) * C::TM + rank * IM + quarter * 32;
+            const int n0 = tn * C::TN + half * 128;
+            const uint32_t buf = n & 1u;
+            const float sa = row0 + lane < p.M ? p.a_s[row0 + lane] : 0.f;
+            fetch_scales(p, n0, 128, epi.sb);
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[buf], (n >> 1) & 1u, DEVERR_PART_WAIT));
+            if (!ok) break;
+            tc_fence_after();
+            store_sums<128>(p, &map_c, tmem + (uint32_t(quarter * 32) << 16) + buf * C::TN + half * 128, row0, n0, sa, epi, [&]() {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa(smem_u32(&acc_empty[buf]), 0)) : "memory");
+            });
+        }
+        if (lane == 0) bulk_wait_all();
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                              // neither leaves while the other's copies, MMAs or arrivals may still reach it
+    tc_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+// Products of few tiles: a cluster of S CTAs shares k of one tile; the rank is the part of k.  Rank r owns the rows r, r + S,
+// ... of the tile: every CTA writes its sums of them to its own place in the owner's shared memory (stores to the other
+// SMs that nobody waits for; reading them from there instead took twice as long), and behind one cluster barrier the
+// owner adds them up and stores the result.  What bounds it is the issue of the MMAs, four per 128 bytes of k whatever
+// their size (about 0.28 us), so k is split as far as there are SMs.
+template <int TN>
+struct SplitTile {
+    static constexpr int STAGE = I_ATILE + TN * IKB;
+    static constexpr int STAGES = TN == 128 ? 4 : 6;
+    static constexpr int SUM_OFF = STAGES * STAGE;                 // the ranks' sums of the rows of this CTA
+    static constexpr int BAR_OFF = SUM_OFF + (IM + 8) * TN * 4;    // S * ceil(IM / S) rows at most
+    static constexpr int SMEM = 1024 + BAR_OFF + 256;
+    static constexpr int THREADS = 192;
+    static_assert(SMEM <= 232448 && 4 * int(sizeof(EpiWarp)) <= SUM_OFF && TN <= EpiWarp::COLS, "shared memory");
+};
+
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, uint4 v) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa(addr, rank)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 template <int TN>
 __global__ void __launch_bounds__(SplitTile<TN>::THREADS)
-int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Int8Params p, int S) {
+int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Int8Params p, int S) {
     using C = SplitTile<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -445,6 +692,7 @@ int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(slot);
+    if (S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");     // waited for before the first store to another CTA
     bool ok = true;
     if (warp == 0) {
         // the weights of the first stages do not depend on the kernel before this one
@@ -498,55 +746,65 @@ int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
     tc_fence_after();
     const int quarter = warp & 3;
     if (S == 1) {
-        if (warp >= 2 && have) {
-            const int64_t row = int64_t(m0) + quarter * 32 + lane;
-            const float sa = row < p.M ? p.a_s[row] : 0.f;
+        if (warp >= 2 && __all_sync(0xffffffffu, have) && int64_t(m0) + quarter * 32 < p.M) {
+            // the stages are free, the scales and the turning room take their place
+            EpiWarp& epi = reinterpret_cast<EpiWarp*>(smem)[warp - 2];
+            const int64_t row0 = int64_t(m0) + quarter * 32;
+            const float sa = row0 + lane < p.M ? p.a_s[row0 + lane] : 0.f;
+            fetch_scales(p, n0, TN, epi.sb);
+            store_sums<TN>(p, &map_c, tmem + (uint32_t(quarter * 32) << 16), row0, n0, sa, epi, []() {});
+            if (lane == 0) bulk_wait_all();
+            __syncwarp();
+        }
+    } else {
+        // place of the sums of rank k for the owner's i-th row: ((k * per + i) * TN) floats, its 16-byte pieces xor-ed with the
+        // row against bank conflicts
+        const int per = (IM + S - 1) / S;
+        const uint32_t sums = smem_u32(smem + C::SUM_OFF);
+        __syncwarp();
+        cluster_wait();                                      // every CTA of the cluster has started: its shared memory is there
+        if (warp >= 2 && __all_sync(0xffffffffu, have) && int64_t(m0) + quarter * 32 < p.M) {   // whole warps without a row of c keep out
+            const int r = quarter * 32 + lane, owner = r % S, i = r / S;
+            const uint32_t at = sums + uint32_t((rank * per + i) * TN * 4);
 #pragma unroll 1
             for (int c = 0; c < TN; c += 32) {
                 uint32_t v[32];
                 tmem_ld_row32(tmem + (uint32_t(quarter * 32) << 16) + c, v);
-                store_row<32>(p, row, n0 + c, v, sa);
-            }
-        }
-    } else {
-        const uint32_t part = smem_u32(smem);
-        if (warp >= 2 && __all_sync(0xffffffffu, have)) {
-            const int r = quarter * 32 + lane;
-            if (int64_t(m0) + quarter * 32 < p.M) {          // whole warps without a row of c keep out
-#pragma unroll 1
-                for (int c = 0; c < TN; c += 32) {
-                    uint32_t v[32];
-                    tmem_ld_row32(tmem + (uint32_t(quarter * 32) << 16) + c, v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {            // 16-byte pieces, xor-ed with the row against bank conflicts
-                        const uint32_t at = uint32_t(r * TN * 4) + ((uint32_t(c / 4 + i) ^ uint32_t(r & 7)) << 4);
-                        *reinterpret_cast<uint4*>(smem + at) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    }
-                }
+                for (int j = 0; j < 8; ++j)
+                    st_cluster(at + ((uint32_t(c / 4 + j) ^ uint32_t(i & 7)) << 4), uint32_t(owner), make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
             }
         }
         __syncwarp();
         cluster_sync();
-        // rank r stores rows r, r + S, ...: 16 columns per thread
-        constexpr int PER = TN / 16;                         // threads per row
         const int rows = int(min(int64_t(IM), p.M - m0));
         const int mine = (rows - rank + S - 1) / S;
-        for (int i = t; i < mine * PER; i += C::THREADS) {
-            const int r = (i / PER) * S + rank, c = (i % PER) * 16;
-            uint32_t v[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = 0u;
+        constexpr int PER = TN / 4;                          // four columns per thread: a warp stores 128 columns of a row
+        for (int q = t; q < mine * PER; q += C::THREADS) {
+            const int i = q / PER, c = (q % PER) * 4, col = n0 + c;
+            uint4 v = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
             for (int k = 0; k < S; ++k) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint4 w = ld_cluster(part + uint32_t(r * TN * 4) + ((uint32_t(c / 4 + j) ^ uint32_t(r & 7)) << 4), uint32_t(k));
-                    v[4 * j] += w.x; v[4 * j + 1] += w.y; v[4 * j + 2] += w.z; v[4 * j + 3] += w.w;
-                }
+                const uint4 w = *reinterpret_cast<const uint4*>(smem + C::SUM_OFF + ((k * per + i) * TN * 4) + ((uint32_t(c / 4) ^ uint32_t(i & 7)) << 4));
+                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
             }
-            store_row<16>(p, int64_t(m0) + r, n0 + c, v, p.a_s[m0 + r]);
+            const int64_t row = int64_t(m0) + i * S + rank;
+            const float sa = p.a_s[row];
+            if (p.wide && col + 4 <= p.N) {
+                const float4 sb = *reinterpret_cast<const float4*>(p.b_s + col);
+                const float f[4] = {__int2float_rn(int(v.x)) * sa * sb.x, __int2float_rn(int(v.y)) * sa * sb.y, __int2float_rn(int(v.z)) * sa * sb.z, __int2float_rn(int(v.w)) * sa * sb.w};
+                const int64_t to = row * p.N + col;
+                if (p.out_dtype == LH_F32) *reinterpret_cast<float4*>(p.c + to * 4) = make_float4(f[0], f[1], f[2], f[3]);
+                else if (p.out_dtype == LH_BF16) *reinterpret_cast<uint2*>(p.c + to * 2) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+                else *reinterpret_cast<uint2*>(p.c + to * 2) = make_uint2(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]));
+            } else {
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (col + j < p.N) store_one(p, row * p.N + col + j, __int2float_rn(int(u[j])) * sa * p.b_s[col + j]);
+            }
         }
-        __syncwarp();
-        cluster_sync();                                      // nobody leaves while others read its sums
     }
     tc_fence_before();
     __syncthreads();
@@ -601,11 +859,42 @@ int int8_check(const char* what, int64_t M, int64_t N, int64_t K, int out_dtype)
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// How many clusters of s CTAs of the split kernel run at once on the current device (asked once per device, tile and s): where
+// there are more of them a second wave doubles the time.
+template <int TN>
+int query_clusters(int s) {
+    using C = SplitTile<TN>;
+    if (cudaFuncSetAttribute(int8_split_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(s));
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(s);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, int8_split_kernel<TN>, &cfg) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    return n;
+}
+int split_clusters(int tn, int s) {
+    static std::atomic<int> known[64][2][9];      // clusters + 1, 0 = not asked
+    int dev = 0;
+    sm_count(&dev);
+    std::atomic<int>* at = dev >= 0 && dev < 64 ? &known[dev][tn == 64][s] : nullptr;
+    if (at && at->load(std::memory_order_relaxed)) return at->load(std::memory_order_relaxed) - 1;
+    const int n = tn == 64 ? query_clusters<64>(s) : query_clusters<128>(s);
+    if (at) at->store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
 // arguments checked, M > 0
 int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
     const int sms = sm_count();
     const int64_t es = p.out_dtype == LH_F32 ? 4 : 2;
-    p.wide = (p.N * es) % 32 == 0 && aligned(p.c, 32) && aligned(p.b_s, 16);
+    p.wide = p.N % 4 == 0 && aligned(p.b_s, 16);
     if (p.M <= 16) {
         const int steps = (p.K + 63) / 64;
         const int warps = std::max(2, std::min(16, (steps + kRowsSteps - 1) / kRowsSteps));
@@ -613,37 +902,63 @@ int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
         if (p.M <= 8) return launch("int8_rows_kernel", int8_rows_kernel<1>, grid, 32u * warps, size_t(warps) * 512, 1, dependent, stream, p);
         return launch("int8_rows_kernel", int8_rows_kernel<2>, grid, 32u * warps, size_t(warps) * 1024, 1, dependent, stream, p);
     }
-    CUtensorMap ma, mb;
+    CUtensorMap ma, mb, mc{};
+    p.mapped = (p.N * es) % 16 == 0;
+    if (p.mapped)
+        if (int rc = make_tensor_map(&mc, p.c, p.out_dtype, uint64_t(p.M), uint64_t(p.N), uint64_t(p.N * es), 32, uint32_t(128 / es), 1)) return rc;
     auto maps = [&](int tn) -> int {
         if (int rc = make_tensor_map(&ma, p.a, LH_U8, uint64_t(p.M), uint64_t(p.K), uint64_t(p.K), IM, IKB, 1)) return rc;
         return make_tensor_map(&mb, p.b, LH_U8, uint64_t(p.N), uint64_t(p.K), uint64_t(p.K), uint32_t(tn), IKB, 1);
     };
-    auto tiles = [&](int tn) { return ceil_div(p.M, IM) * ceil_div(p.N, tn); };
-    if (tiles(256) >= sms) {
-        using C = BigTile<256>;
-        if (int rc = maps(256)) return rc;
-        return launch("int8_tile_kernel", int8_tile_kernel<256>, unsigned(std::min<int64_t>(tiles(256), sms)), C::THREADS, C::SMEM, 1, dependent, stream, ma, mb, p);
+    // Which kernel, by an estimate in microseconds: the slowest CTA's MMAs per 128 bytes of k, at least its stores, or what all
+    // CTAs bring in through L2 at 9.5 TB/s, and what follows the last MMA: the join of a split k, or stores that nothing hides (longest
+    // where rows have to be written element by element).  It follows the measured times within about 2 us plus 4 for
+    // the launch: 32 x 4096 x 4096 8.2 us (128 columns, k in 4; whole 15.1), 300 x 1024 x 8192 13.7 (in 4; 25.0),
+    // 1000 x 1111 x 2064 12.3 (64 columns, whole; 128 columns in 2 14.4), 512 x 4096 x 4096 16.6 (pair; 128 columns 18.1),
+    // 4096 x 8192 x 512 34 (tile; pair 39), 8192 x 8192 x 4096 180 (pair; tile 285).
+    const int kblocks = int(ceil_div(p.K, IKB));
+    enum { SPLIT64, SPLIT128, TILE, PAIR };
+    int kind = PAIR, parts = 1;
+    double best = 1e30;
+    auto consider = [&](int which, int s, int64_t count, int64_t at_once, int nkb, int tm, int tn, double per_block, double stores, double join) {
+        const double rows = double(std::min<int64_t>(p.M, tm));
+        const double mma = double(ceil_div(count, at_once)) * std::max(nkb * per_block, stores);
+        const double l2 = double(count) * s * nkb * IKB * (rows + tn) / 9.5e6;
+        const double cost = std::max(mma, l2) + join;
+        if (cost < best) { best = cost; kind = which; parts = s; }
+    };
+    auto tiles = [&](int tm, int tn) { return ceil_div(p.M, tm) * ceil_div(p.N, tn); };
+    consider(PAIR, 1, tiles(256, 256), sms / 2, kblocks, 256, 256, 0.38, 5.0, p.mapped ? 0.0 : 9.0);
+    if (tiles(IM, 128) > sms) consider(TILE, 1, tiles(IM, 128), sms, kblocks, IM, 128, 0.33, 2.1, p.mapped ? 0.0 : 4.0);
+    for (const int tn : {64, 128}) {
+        const int64_t n = tiles(IM, tn);
+        if (n > sms) continue;
+        const double per_block = tn == 64 ? 0.29 : 0.33;
+        for (const int s : {1, 2, 3, 4, 6, 8})
+            if (s <= kblocks && (s == 1 || n <= split_clusters(tn, s)))
+                consider(tn == 64 ? SPLIT64 : SPLIT128, s, n, n, int(ceil_div(kblocks, s)), IM, tn, per_block, 0.0,
+                         s > 1 ? (tn == 64 ? 0.7 : 1.0) + 0.008 * double(std::min<int64_t>(p.M, IM)) : p.mapped ? (tn == 64 ? 0.9 : 2.0) : tn == 64 ? 2.5 : 6.5);
     }
-    if (tiles(128) >= sms) {
+    if (kind == PAIR) {
+        using C = PairTile;
+        if (int rc = maps(128)) return rc;
+        return launch("int8_pair_kernel", int8_pair_kernel, unsigned(2 * std::min<int64_t>(tiles(256, 256), sms / 2)), C::THREADS, C::SMEM, 2, dependent,
+                      stream, ma, mb, mc, p);
+    }
+    if (kind == TILE) {
         using C = BigTile<128>;
         if (int rc = maps(128)) return rc;
-        return launch("int8_tile_kernel", int8_tile_kernel<128>, unsigned(std::min<int64_t>(tiles(128), sms)), C::THREADS, C::SMEM, 1, dependent, stream, ma, mb, p);
+        return launch("int8_tile_kernel", int8_tile_kernel<128>, unsigned(std::min<int64_t>(tiles(IM, 128), sms)), C::THREADS, C::SMEM, 1, dependent, stream,
+                      ma, mb, mc, p);
     }
-    const int kblocks = int(ceil_div(p.K, IKB));
-    auto split = [&](int tn) {
-        int s = 1;
-        while (s < 8 && tiles(tn) * s * 2 <= sms && kblocks / (s * 2) >= 2) s *= 2;
-        return s;
-    };
     auto go = [&](auto tag) {
         constexpr int TN = decltype(tag)::value;
         using C = SplitTile<TN>;
         if (int rc = maps(TN)) return rc;
-        const int s = split(TN);
-        return launch("int8_split_kernel", int8_split_kernel<TN>, unsigned(tiles(TN) * s), C::THREADS, C::SMEM, unsigned(s), dependent, stream, ma, mb, p, s);
+        return launch("int8_split_kernel", int8_split_kernel<TN>, unsigned(tiles(IM, TN) * parts), C::THREADS, C::SMEM, unsigned(parts), dependent, stream, ma, mb,
+                      mc, p, parts);
     };
-    if (tiles(64) <= sms / 2) return go(std::integral_constant<int, 64>{});
-    return go(std::integral_constant<int, 128>{});
+    return kind == SPLIT64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
 }
 
 int token_launch(TokenParams p, int dtype, cudaStream_t stream) {
