@@ -8,7 +8,10 @@ from __future__ import annotations
 
 import torch
 
-from linghe_b200.utils.norm import (triton_rms_norm_and_block_quant_forward, triton_rms_norm_backward,
+from torch.autograd.function import once_differentiable
+
+from linghe_b200.utils.norm import (rms_norm_pair_backward, rms_norm_pair_forward,
+                                    triton_rms_norm_and_block_quant_forward, triton_rms_norm_backward,
                                     triton_rms_norm_forward)
 
 
@@ -88,3 +91,37 @@ def block_rms_norm(input, weight, rms, quantizer, cls, eps=1e-6, is_recomputing=
     """linghe/facade/norm.py:107."""
     output, output_rms = BlockRMSNorm.apply(input, weight, rms, eps, quantizer, cls, is_recomputing)
     return output, output_rms.detach()
+
+
+class RMSNormPair(torch.autograd.Function):
+    """The norm after a block, gate, residual scale, residual sum and the norm before the next block, with the fused
+    backward.  Saves o and h -- or their 8-bit checkpoints -- and 1/rms of both."""
+
+    @staticmethod
+    def forward(ctx, x, o, post_weight, pre_weight, gate, residual_scale, eps, checkpoint):
+        h, y, rms_post, rms_pre, saved = rms_norm_pair_forward(x, o, post_weight, pre_weight, gate, residual_scale, eps, checkpoint)
+        o_kept, o_scale, h_kept, h_scale = (o, None, h, None) if saved is None else saved
+        ctx.save_for_backward(o_kept, o_scale, h_kept, h_scale, post_weight, pre_weight, gate, rms_post, rms_pre)
+        ctx.residual_scale = residual_scale
+        ctx.set_materialize_grads(False)
+        return h, y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, grad_y):
+        o, o_scale, h, h_scale, post_weight, pre_weight, gate, rms_post, rms_pre = ctx.saved_tensors
+        if grad_h is None and grad_y is None:
+            return (None,) * 8
+        if grad_y is None:        # the second norm leads nowhere
+            grad_y = torch.zeros_like(grad_h)
+        dx, do, dpost, dpre, dgate = rms_norm_pair_backward(
+            grad_y.contiguous(), None if grad_h is None else grad_h.contiguous(), o, h, post_weight, pre_weight, rms_post, rms_pre,
+            gate, ctx.residual_scale, o_scale, h_scale)
+        return dx, do, dpost, dpre, dgate, None, None, None
+
+
+def rms_norm_pair(x, o, post_weight, pre_weight, gate=None, residual_scale=1.0, eps=1e-6, checkpoint=None):
+    """(h, y) with h = x + residual_scale * gate * RMSNorm(o) * post_weight and y = RMSNorm(h) * pre_weight, differentiable
+    in x, o, both weights and the gate.  See linghe_b200.utils.norm.rms_norm_pair_forward for shapes; `checkpoint`
+    (torch.int8 or torch.float8_e4m3fn) keeps o and h for the backward pass in 8 bits."""
+    return RMSNormPair.apply(x, o, post_weight, pre_weight, gate, residual_scale, eps, checkpoint)

@@ -5,8 +5,10 @@ linghe/facade/silu.py.  ``cls`` is the injected FP8 tensor container; quantizers
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from linghe_b200.utils.silu import (triton_batch_weighted_silu_and_block_quant_backward,
+from linghe_b200.utils.silu import (silu_and_checkpoint_backward, silu_and_checkpoint_forward,
+                                    triton_batch_weighted_silu_and_block_quant_backward,
                                     triton_batch_weighted_silu_and_block_quant_forward,
                                     triton_silu_and_block_quant_backward,
                                     triton_silu_and_block_quant_forward)
@@ -100,3 +102,31 @@ def block_batch_weighted_silu_impl(input, weights, counts, splits, quantizers, g
     assert input.ndim == 2
     return BlockBatchWeightedSiluFunction.apply(input, weights, counts, splits, quantizers, grad_quantizers,
                                                 cls, is_recomputing)
+
+
+class CheckpointedSilu(torch.autograd.Function):
+    """SwiGLU that saves an 8-bit checkpoint of its input in place of the input."""
+
+    @staticmethod
+    def forward(ctx, input, weight, checkpoint):
+        shape = input.shape
+        rows = input.reshape(-1, shape[-1])
+        out, x_q, x_scale = silu_and_checkpoint_forward(rows, None if weight is None else weight.reshape(-1), checkpoint)
+        ctx.save_for_backward(x_q, x_scale, weight)
+        ctx.shape = shape
+        return out.view(*shape[:-1], shape[-1] // 2)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        x_q, x_scale, weight = ctx.saved_tensors
+        g = grad_output.contiguous().view(-1, grad_output.shape[-1])
+        dx, dw = silu_and_checkpoint_backward(g, x_q, x_scale, None if weight is None else weight.reshape(-1))
+        return dx.view(ctx.shape), None if dw is None else dw.view(weight.shape), None
+
+
+def checkpointed_silu(input, weight=None, checkpoint=torch.int8):
+    """silu(x1) * x2 [* weight] for input [..., 2n] = [x1 | x2], contiguous, differentiable in input and weight (one float32 or
+    bf16 value per row).  Between the passes input is kept as 8-bit codes (torch.int8 or torch.float8_e4m3fn)."""
+    assert input.is_contiguous()
+    return CheckpointedSilu.apply(input, weight, checkpoint)
