@@ -157,7 +157,7 @@ def _build_host(verbose: bool) -> None:
                "-I" + os.path.join(os.path.dirname(PKG), "include"), "-I" + OBJDIR, "-I/usr/local/cuda/include",
                "-I" + sysconfig.get_paths()["include"], *["-I" + d for d in ce.include_paths()],
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_lh_host",
-               "-DTORCH_API_INCLUDE_EXTENSION_H", "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+               "-DTORCH_API_INCLUDE_EXTENSION_H", "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
                "-ltorch_python", "-L" + LIBDIR, "-llinghe_b200", "-Wl,-rpath,$ORIGIN"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:

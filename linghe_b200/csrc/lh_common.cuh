@@ -10,6 +10,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/linghe_b200.h"
 
 namespace lh {
@@ -21,6 +23,19 @@ void set_error(const char* fmt, ...);
 int fail_arg(const char* fmt, ...);      // records message, returns LH_ERR_ARG
 int check_launch(const char* what);      // cudaGetLastError -> status code
 int sm_count(int* out_device = nullptr); // SM count of the current device (cached)
+// Allows a kernel `bytes` of dynamic shared memory, once per device.
+template <auto KERN>
+int allow_smem(int bytes) {
+    static std::atomic<uint64_t> allowed{0};       // a bit per device
+    int dev = 0;
+    sm_count(&dev);
+    const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+    if (allowed.load(std::memory_order_relaxed) & bit) return LH_OK;
+    const cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) { (void)cudaGetLastError(); set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return int(e); }
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+    return LH_OK;
+}
 // Tiled 2-D tensor map over a row-major [rows, cols] matrix with `pitch_bytes` between
 // rows; the box is box_rows x box_cols elements, out-of-range reads give 0.  swizzle128:
 // lay the box out with the 128-byte swizzle (box rows must then be 128 bytes long).

@@ -813,14 +813,11 @@ int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
 
 // one launch: `dependent` lets it start while the kernel before it in the stream still runs (the kernels here wait for that
 // kernel before they touch what it writes), `cluster` CTAs share distributed shared memory
-template <typename T> struct Same { using type = T; };   // keeps an argument out of the deduction
-template <typename... Args>
-int launch(const char* what, void (*kern)(Args...), unsigned grid, unsigned block, size_t smem, unsigned cluster, bool dependent,
-           cudaStream_t stream, typename Same<Args>::type... args) {
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-        if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return int(e); }
-    }
+template <auto KERN, typename... Args>
+int launch(const char* what, unsigned grid, unsigned block, size_t smem, unsigned cluster, bool dependent,
+           cudaStream_t stream, const Args&... args) {
+    if (smem > 48 * 1024)                        // a constant of the kernel
+        if (int rc = allow_smem<KERN>(int(smem))) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
@@ -841,7 +838,7 @@ int launch(const char* what, void (*kern)(Args...), unsigned grid, unsigned bloc
     }
     cfg.attrs = attr;
     cfg.numAttrs = unsigned(n);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, KERN, args...);
     if (e != cudaSuccess) { (void)cudaGetLastError(); set_error("%s: %s", what, cudaGetErrorString(e)); return int(e); }
     return LH_OK;
 }
@@ -864,7 +861,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 template <int TN>
 int query_clusters(int s) {
     using C = SplitTile<TN>;
-    if (cudaFuncSetAttribute(int8_split_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (allow_smem<int8_split_kernel<TN>>(C::SMEM) != LH_OK) return 0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(s));
     cfg.blockDim = dim3(C::THREADS);
@@ -899,8 +896,8 @@ int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
         const int steps = (p.K + 63) / 64;
         const int warps = std::max(2, std::min(16, (steps + kRowsSteps - 1) / kRowsSteps));
         const unsigned grid = unsigned(ceil_div(p.N, 16));
-        if (p.M <= 8) return launch("int8_rows_kernel", int8_rows_kernel<1>, grid, 32u * warps, size_t(warps) * 512, 1, dependent, stream, p);
-        return launch("int8_rows_kernel", int8_rows_kernel<2>, grid, 32u * warps, size_t(warps) * 1024, 1, dependent, stream, p);
+        if (p.M <= 8) return launch<int8_rows_kernel<1>>("int8_rows_kernel", grid, 32u * warps, size_t(warps) * 512, 1, dependent, stream, p);
+        return launch<int8_rows_kernel<2>>("int8_rows_kernel", grid, 32u * warps, size_t(warps) * 1024, 1, dependent, stream, p);
     }
     CUtensorMap ma, mb, mc{};
     p.mapped = (p.N * es) % 16 == 0;
@@ -942,20 +939,20 @@ int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
     if (kind == PAIR) {
         using C = PairTile;
         if (int rc = maps(128)) return rc;
-        return launch("int8_pair_kernel", int8_pair_kernel, unsigned(2 * std::min<int64_t>(tiles(256, 256), sms / 2)), C::THREADS, C::SMEM, 2, dependent,
+        return launch<int8_pair_kernel>("int8_pair_kernel", unsigned(2 * std::min<int64_t>(tiles(256, 256), sms / 2)), C::THREADS, C::SMEM, 2, dependent,
                       stream, ma, mb, mc, p);
     }
     if (kind == TILE) {
         using C = BigTile<128>;
         if (int rc = maps(128)) return rc;
-        return launch("int8_tile_kernel", int8_tile_kernel<128>, unsigned(std::min<int64_t>(tiles(IM, 128), sms)), C::THREADS, C::SMEM, 1, dependent, stream,
+        return launch<int8_tile_kernel<128>>("int8_tile_kernel", unsigned(std::min<int64_t>(tiles(IM, 128), sms)), C::THREADS, C::SMEM, 1, dependent, stream,
                       ma, mb, mc, p);
     }
     auto go = [&](auto tag) {
         constexpr int TN = decltype(tag)::value;
         using C = SplitTile<TN>;
         if (int rc = maps(TN)) return rc;
-        return launch("int8_split_kernel", int8_split_kernel<TN>, unsigned(tiles(IM, TN) * parts), C::THREADS, C::SMEM, unsigned(parts), dependent, stream, ma, mb,
+        return launch<int8_split_kernel<TN>>("int8_split_kernel", unsigned(tiles(IM, TN) * parts), C::THREADS, C::SMEM, unsigned(parts), dependent, stream, ma, mb,
                       mc, p, parts);
     };
     return kind == SPLIT64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
@@ -969,11 +966,15 @@ int token_launch(TokenParams p, int dtype, cudaStream_t stream) {
     const int team = hold ? int(warps) : kTokWarps, teams = std::max(1, 4 / team);
     const int64_t grid = ceil_div(p.M, teams);
     if (grid > 0x7fffffff) return fail_arg("token_quant_int8: too many rows");
-    auto go = [&](auto kern) { return launch("token_quant_kernel", kern, unsigned(grid), 32u * team * teams, 0, 1, false, stream, p, team); };
+    const unsigned threads = 32u * team * teams;
+    const char* what = "token_quant_kernel";
     auto with = [&](auto type) {
         using T = decltype(type);
-        if (p.smooth) return hold ? go(token_quant_kernel<T, true, true>) : go(token_quant_kernel<T, false, true>);
-        return hold ? go(token_quant_kernel<T, true, false>) : go(token_quant_kernel<T, false, false>);
+        if (p.smooth)
+            return hold ? launch<token_quant_kernel<T, true, true>>(what, unsigned(grid), threads, 0, 1, false, stream, p, team)
+                        : launch<token_quant_kernel<T, false, true>>(what, unsigned(grid), threads, 0, 1, false, stream, p, team);
+        return hold ? launch<token_quant_kernel<T, true, false>>(what, unsigned(grid), threads, 0, 1, false, stream, p, team)
+                    : launch<token_quant_kernel<T, false, false>>(what, unsigned(grid), threads, 0, 1, false, stream, p, team);
     };
     if (dtype == LH_BF16) return with(__nv_bfloat16{});
     if (dtype == LH_F16) return with(__half{});

@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kPairMaxN = 8192;
 constexpr int kPairMaxThreads = kPairMaxN / 16;
+constexpr int kPairThreadsPerSm = 512;     // backward, 128 registers a thread
 constexpr int kPairMaxStages = 4;
 constexpr int kPairSmem = 227 * 1024;      // shared memory of an SM that CTAs can ask for
 constexpr int kPairSlack = 5120;           // per CTA: static shared memory, what the system reserves, rounding
@@ -597,11 +598,12 @@ __global__ void __launch_bounds__(256) pair_reduce_kernel(const float* part, int
     }
 }
 
+// The backward kernel wants 128 registers a thread, so 512 threads fill an SM: CTAs of rows of up to 4096 columns share it, wider
+// ones are alone on it.  (Two CTAs of 320 threads with 96 registers each spill: 86 us instead of 73 at 5005 x 5120, int8.)
 int pair_threads(int64_t n) { return int((n / 16 + 31) / 32 * 32); }
-
-// CTAs per SM and stages of `bytes` each, with `fixed` bytes beside them: `threads` in all on an SM, at least two stages
-void pair_shape(int threads_per_sm, int nt, int64_t bytes, int64_t fixed, int& per_sm, int& stages) {
-    per_sm = std::max(1, std::min(32, threads_per_sm / nt));
+int pair_per_sm(int64_t n) { return std::max(1, std::min(32, kPairThreadsPerSm / pair_threads(n))); }
+// Stages of `bytes` each, with `fixed` bytes beside them; fewer CTAs per SM where there is no room for two stages
+void pair_shape(int64_t bytes, int64_t fixed, int& per_sm, int& stages) {
     while (true) {
         stages = int(std::min<int64_t>(kPairMaxStages, (kPairSmem / per_sm - kPairSlack - fixed) / bytes));
         if (stages >= 2 || per_sm == 1) break;
@@ -610,28 +612,27 @@ void pair_shape(int threads_per_sm, int nt, int64_t bytes, int64_t fixed, int& p
     stages = std::max(stages, 1);
 }
 
-constexpr int kPairThreadsPerSm = 512;   // 128 registers a thread
 
-template <typename F>
-int pair_launch(F kern, int64_t grid, int nt, int64_t smem, const PairParams& p, const char* what, cudaStream_t stream) {
-    if (smem > 0) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-        if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return int(e); }
-    }
-    kern<<<unsigned(grid), nt, size_t(smem), stream>>>(p);
+template <void (*KERN)(PairParams)>
+int pair_launch(int64_t grid, int nt, int64_t smem, const PairParams& p, const char* what, cudaStream_t stream) {
+    // the same limit for every call: another thread's launch of this kernel with other sizes may come in between
+    if (smem > 0)
+        if (int rc = allow_smem<KERN>(kPairSmem - kPairSlack)) return rc;
+    KERN<<<unsigned(grid), nt, size_t(smem), stream>>>(p);
     return check_launch(what);
 }
 
 template <typename T>
 int pair_fwd_typed(const PairParams& p, int ck, cudaStream_t stream) {
-    auto go = [&](auto kern) { return pair_launch(kern, p.M, int((p.n * sizeof(T) / 32 + 31) / 32 * 32), 0, p, "pair_fwd_kernel", stream); };
-    if (ck == CODES_INT8) return go(pair_fwd_kernel<T, CODES_INT8>);
-    if (ck == CODES_E4M3) return go(pair_fwd_kernel<T, CODES_E4M3>);
-    return go(pair_fwd_kernel<T, CODES_NONE>);
+    const int nt = int((p.n * sizeof(T) / 32 + 31) / 32 * 32);
+    const char* what = "pair_fwd_kernel";
+    if (ck == CODES_INT8) return pair_launch<pair_fwd_kernel<T, CODES_INT8>>(p.M, nt, 0, p, what, stream);
+    if (ck == CODES_E4M3) return pair_launch<pair_fwd_kernel<T, CODES_E4M3>>(p.M, nt, 0, p, what, stream);
+    return pair_launch<pair_fwd_kernel<T, CODES_NONE>>(p.M, nt, 0, p, what, stream);
 }
 
 int64_t pair_bwd_grid(int64_t M, int64_t n) {
-    return std::min<int64_t>(M, int64_t(sm_count()) * std::max(1, std::min(32, kPairThreadsPerSm / pair_threads(n))));
+    return std::min<int64_t>(M, int64_t(sm_count()) * pair_per_sm(n));
 }
 
 template <typename T>
@@ -640,17 +641,19 @@ int pair_bwd_typed(PairParams& p, int ck, float* dpost, float* dpre, cudaStream_
     const int64_t code = ck == CODES_NONE ? int64_t(sizeof(T)) : 1;
     const bool each = p.gate && p.G == p.M && p.M > 1, groups = p.gate && p.G > 1 && !each;
     const int64_t bytes = p.n * (int64_t(sizeof(T)) * (1 + (p.dh ? 1 : 0) + (each ? 1 : 0)) + 2 * code);
-    int per_sm;
+    int per_sm = pair_per_sm(p.n);
     const int64_t fixed = groups ? int64_t(nt) * 64 : 0;
-    pair_shape(kPairThreadsPerSm, nt, bytes, fixed, per_sm, p.stages);
+    pair_shape(bytes, fixed, per_sm, p.stages);
     const int64_t grid = std::min(pair_bwd_grid(p.M, p.n), int64_t(sm_count()) * per_sm);
-    auto go = [&](auto kern) { return pair_launch(kern, grid, nt, bytes * p.stages + fixed, p, "pair_bwd_kernel", stream); };
+    const int64_t smem = bytes * p.stages + fixed;
+    const char* what = "pair_bwd_kernel";
     int rc;
     auto with = [&](auto codes) {
         constexpr int CK = decltype(codes)::value;
-        if (!p.gate) return go(pair_bwd_kernel<T, CK, GATE_NONE>);
-        if (p.G == 1) return go(pair_bwd_kernel<T, CK, GATE_ROW>);
-        return each ? go(pair_bwd_kernel<T, CK, GATE_EACH>) : go(pair_bwd_kernel<T, CK, GATE_GROUPS>);
+        if (!p.gate) return pair_launch<pair_bwd_kernel<T, CK, GATE_NONE>>(grid, nt, smem, p, what, stream);
+        if (p.G == 1) return pair_launch<pair_bwd_kernel<T, CK, GATE_ROW>>(grid, nt, smem, p, what, stream);
+        return each ? pair_launch<pair_bwd_kernel<T, CK, GATE_EACH>>(grid, nt, smem, p, what, stream)
+                    : pair_launch<pair_bwd_kernel<T, CK, GATE_GROUPS>>(grid, nt, smem, p, what, stream);
     };
     if (ck == CODES_INT8) rc = with(std::integral_constant<int, CODES_INT8>{});
     else if (ck == CODES_E4M3) rc = with(std::integral_constant<int, CODES_E4M3>{});

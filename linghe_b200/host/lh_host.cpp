@@ -8,6 +8,7 @@
 // (linghe/utils/norm.py:343-502, linghe/utils/silu.py:279-335).
 #include <torch/extension.h>
 
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -165,6 +166,12 @@ void check_same(const at::Tensor& ref, at::ScalarType type, const char* name, co
     if (t.sizes() != shape) raise_assert(std::string(name) + " has another shape than expected");
 }
 
+// an uninitialised tensor on the device of `ref`, straight from the CUDA allocator (the dispatcher in front of at::empty costs
+// as much as the allocation)
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& ref) {
+    return at::detail::empty_cuda(sizes, type, ref.device(), std::nullopt);
+}
+
 const void* cptr(const OptT& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 float* fptr(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
 const float* fptr(const OptT& t) { return t.has_value() ? static_cast<const float*>(t->data_ptr()) : nullptr; }
@@ -212,14 +219,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, Saved> rms_norm_pair_
     if (gate.has_value()) check_same(x, type, "gate", *gate);
     const int64_t G = gate_rows(gate, x);
     const c10::cuda::OptionalCUDAGuard guard(x.device());
-    const auto f32 = x.options().dtype(at::kFloat);
-    const at::Tensor h = at::empty(x.sizes(), x.options()), y = at::empty(x.sizes(), x.options()), rp = at::empty({M}, f32), rh = at::empty({M}, f32);
+    const at::Tensor h = fresh(x.sizes(), x.scalar_type(), x), y = fresh(x.sizes(), x.scalar_type(), x), rp = fresh({M}, at::kFloat, x), rh = fresh({M}, at::kFloat, x);
     Saved saved;
     at::Tensor oq, os, hq, hs;
     if (codes) {
-        const auto q = x.options().dtype(*checkpoint);
-        oq = at::empty(x.sizes(), q); os = at::empty({M, n / 128}, f32);
-        hq = at::empty(x.sizes(), q); hs = at::empty({M, n / 128}, f32);
+        oq = fresh(x.sizes(), *checkpoint, x); os = fresh({M, n / 128}, at::kFloat, x);
+        hq = fresh(x.sizes(), *checkpoint, x); hs = fresh({M, n / 128}, at::kFloat, x);
         saved = std::make_tuple(oq, os, hq, hs);
     }
     check_rc(lh_rmsnorm_pair_fwd(x.data_ptr(), o.data_ptr(), post.data_ptr(), pre.data_ptr(), cptr(gate), dt, M, n, G, float(alpha), float(eps),
@@ -254,12 +259,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, OptT> rms_norm_pair_b
     if (gate.has_value()) check_same(dy, type, "gate", *gate);
     const int64_t G = gate_rows(gate, dy);
     const c10::cuda::OptionalCUDAGuard guard(dy.device());
-    const auto f32 = dy.options().dtype(at::kFloat);
     const int64_t nbytes = lh_scratch_bytes("rmsnorm_pair_bwd", M, n);
-    const at::Tensor dx = at::empty(dy.sizes(), dy.options()), dout = at::empty(dy.sizes(), dy.options()), dpost = at::empty({n}, f32),
-                     dpre = at::empty({n}, f32), scratch = at::empty({nbytes}, dy.options().dtype(at::kByte));
+    const at::Tensor dx = fresh(dy.sizes(), dy.scalar_type(), dy), dout = fresh(dy.sizes(), dy.scalar_type(), dy), dpost = fresh({n}, at::kFloat, dy),
+                     dpre = fresh({n}, at::kFloat, dy), scratch = fresh({nbytes}, at::kByte, dy);
     OptT dgate;
-    if (gate.has_value()) dgate = at::empty(gate->sizes(), dy.options());
+    if (gate.has_value()) dgate = fresh(gate->sizes(), dy.scalar_type(), dy);
     check_rc(lh_rmsnorm_pair_bwd(dy.data_ptr(), cptr(dh), o.data_ptr(), fptr(os), h.data_ptr(), fptr(hs), post.data_ptr(), pre.data_ptr(),
                                  cptr(gate), fptr(rp), fptr(rh), dt, M, n, G, float(alpha), codes, dx.data_ptr(), dout.data_ptr(), fptr(dpost),
                                  fptr(dpre), ptr(dgate), scratch.data_ptr(), nbytes, c10::cuda::getCurrentCUDAStream().stream()),
@@ -284,8 +288,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> silu_and_checkpoint_forward(const
     check_same(x, x.scalar_type(), "x", x);
     const int wt = weight_code(x, w, M);
     const c10::cuda::OptionalCUDAGuard guard(x.device());
-    const at::Tensor y = at::empty({M, N / 2}, x.options()), q = at::empty({M, N}, x.options().dtype(*checkpoint)),
-                     s = at::empty({M, N / 128}, x.options().dtype(at::kFloat));
+    const at::Tensor y = fresh({M, N / 2}, x.scalar_type(), x), q = fresh({M, N}, *checkpoint, x),
+                     s = fresh({M, N / 128}, at::kFloat, x);
     check_rc(lh_silu_checkpoint_fwd(x.data_ptr(), cptr(w), dt, wt, codes, M, N / 2, y.data_ptr(), q.data_ptr(), fptr(s),
                                     c10::cuda::getCurrentCUDAStream().stream()),
              "lh_silu_checkpoint_fwd");
@@ -303,9 +307,9 @@ std::tuple<at::Tensor, OptT> silu_and_checkpoint_backward(const at::Tensor& g, c
     check_same(g, at::kFloat, "x_scale", s, {M, N / 128});
     const int wt = weight_code(g, w, M);
     const c10::cuda::OptionalCUDAGuard guard(g.device());
-    const at::Tensor dx = at::empty({M, N}, g.options());
+    const at::Tensor dx = fresh({M, N}, g.scalar_type(), g);
     OptT dw;
-    if (w.has_value()) dw = at::empty({M}, w->options());
+    if (w.has_value()) dw = fresh({M}, w->scalar_type(), *w);
     check_rc(lh_silu_checkpoint_bwd(g.data_ptr(), q.data_ptr(), fptr(s), cptr(w), dt, wt, codes, M, N / 2, dx.data_ptr(), ptr(dw),
                                     c10::cuda::getCurrentCUDAStream().stream()),
              "lh_silu_checkpoint_bwd");
@@ -327,8 +331,8 @@ std::tuple<at::Tensor, at::Tensor> token_quant_int8(const at::Tensor& x, const O
     check_same(x, x.scalar_type(), "x", x);
     if (smooth.has_value()) check_same(x, at::kFloat, "smooth_scale", *smooth, {K});
     const c10::cuda::OptionalCUDAGuard guard(x.device());
-    if (!out.has_value()) out = at::empty(x.sizes(), x.options().dtype(at::kChar));
-    if (!scale.has_value()) scale = at::empty({M}, x.options().dtype(at::kFloat));
+    if (!out.has_value()) out = fresh(x.sizes(), at::kChar, x);
+    if (!scale.has_value()) scale = fresh({M}, at::kFloat, x);
     check_same(x, at::kChar, "out", *out, x.sizes());
     check_same(x, at::kFloat, "scale", *scale, {M});
     check_rc(lh_token_quant_int8(x.data_ptr(), fptr(smooth), dt, M, K, out->data_ptr(), fptr(*scale), c10::cuda::getCurrentCUDAStream().stream()),
@@ -357,7 +361,7 @@ at::Tensor int8_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor&
     check_same(a, at::kFloat, "a_s", a_s, {M});
     check_same(a, at::kFloat, "b_s", b_s, {N});
     const c10::cuda::OptionalCUDAGuard guard(a.device());
-    const at::Tensor c = at::empty(last_dim(a, N), a.options().dtype(out_dtype));
+    const at::Tensor c = fresh(last_dim(a, N), out_dtype, a);
     check_rc(lh_int8_gemm(a.data_ptr(), b.data_ptr(), fptr(a_s), fptr(b_s), c.data_ptr(), M, N, K, od, c10::cuda::getCurrentCUDAStream().stream()),
              "lh_int8_gemm");
     return c;
@@ -376,8 +380,8 @@ at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tenso
     check_same(x, at::kFloat, "w_s", w_s, {N});
     if (smooth.has_value()) check_same(x, at::kFloat, "smooth_scale", *smooth, {K});
     const c10::cuda::OptionalCUDAGuard guard(x.device());
-    const at::Tensor c = at::empty(last_dim(x, N), x.options().dtype(type));
-    const at::Tensor ws = at::empty({M * K + 4 * M}, x.options().dtype(at::kByte));      // codes, then scales: K is a multiple of 16
+    const at::Tensor c = fresh(last_dim(x, N), type, x);
+    const at::Tensor ws = fresh({M * K + 4 * M}, at::kByte, x);      // codes, then scales: K is a multiple of 16
     uint8_t* q = static_cast<uint8_t*>(ws.data_ptr());
     check_rc(lh_int8_linear(x.data_ptr(), fptr(smooth), dt, w.data_ptr(), fptr(w_s), q, reinterpret_cast<float*>(q + M * K), c.data_ptr(), M, N, K,
                             od, c10::cuda::getCurrentCUDAStream().stream()),
