@@ -404,8 +404,9 @@ int lh_int8_gemm(const void* a, const void* b, const float* a_s, const float* b_
                  int64_t K, int out_dtype, void* stream);
 
 /* The two above in one call: c = x b^T with x [M,K] of `dtype` quantised per token into the workspaces
- * q [M,K] (int8) and s [M] (float32), which hold the codes and scales afterwards.  The product starts while the
- * quantiser still runs and waits for it on the device. */
+ * q [M,K] (int8) and s [M] (float32), which hold the codes and scales afterwards.  One kernel for one token
+ * and a few thousand channels; else the product starts while the quantiser still runs and waits for it on
+ * the device. */
 int lh_int8_linear(const void* x, const float* smooth, int dtype, const void* b, const float* b_s, void* q, float* s,
                    void* c, int64_t M, int64_t N, int64_t K, int out_dtype, void* stream);
 

@@ -35,6 +35,17 @@ struct TokenParams {
     float* s;
 };
 
+// eight elements over max(smooth, 1e-30)
+__device__ __forceinline__ void smooth8(const float* smooth, float2* e) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float4 m = *reinterpret_cast<const float4*>(smooth + 4 * h);
+        float2 &lo = e[2 * h], &hi = e[2 * h + 1];
+        lo = make_float2(__fdiv_rn(lo.x, max_nan(m.x, kScaleFloor)), __fdiv_rn(lo.y, max_nan(m.y, kScaleFloor)));
+        hi = make_float2(__fdiv_rn(hi.x, max_nan(m.z, kScaleFloor)), __fdiv_rn(hi.y, max_nan(m.w, kScaleFloor)));
+    }
+}
+
 // the elements at column c over max(smooth, 1e-30)
 template <typename T>
 __device__ __forceinline__ void smoothed(const Lane<T>& x, const float* smooth, int c, float2 (&e)[Lane<T>::V][4]) {
@@ -42,13 +53,7 @@ __device__ __forceinline__ void smoothed(const Lane<T>& x, const float* smooth, 
     for (int v = 0; v < Lane<T>::V; ++v) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[v][i] = x.v[v].get(i);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float4 m = *reinterpret_cast<const float4*>(smooth + c + 8 * v + 4 * h);
-            float2 &lo = e[v][2 * h], &hi = e[v][2 * h + 1];
-            lo = make_float2(__fdiv_rn(lo.x, max_nan(m.x, kScaleFloor)), __fdiv_rn(lo.y, max_nan(m.y, kScaleFloor)));
-            hi = make_float2(__fdiv_rn(hi.x, max_nan(m.z, kScaleFloor)), __fdiv_rn(hi.y, max_nan(m.w, kScaleFloor)));
-        }
+        smooth8(smooth + c + 8 * v, e[v]);
     }
 }
 
@@ -204,22 +209,14 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NT>
-__global__ void __launch_bounds__(512) int8_rows_kernel(const Int8Params p) {
-    extern __shared__ int red[];                     // [warps][NT][16][8]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int g = lane >> 2, tig = lane & 3;
-    const int n0 = blockIdx.x * 16;
-    const bool r0 = n0 + g < p.N, r1 = n0 + g + 8 < p.N;
-    const uint8_t* b0 = p.b + int64_t(n0 + g) * p.K;
-    const uint8_t* b1 = b0 + int64_t(8) * p.K;
-    const int steps = (p.K + 63) >> 6;
-    int acc[NT][4];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0;
-    bool waited = false;
-    for (int s0 = warp; s0 < steps; s0 += warps * kRowsSteps) {
-        uint4 w0[kRowsSteps], w1[kRowsSteps];
+// A warp's weights of steps s0, s0 + warps, ...: 16 bytes of two channels per lane and step.
+struct RowWeights {
+    uint4 w0[kRowsSteps], w1[kRowsSteps];
+    __device__ __forceinline__ void load(const Int8Params& p, int n0, int s0, int warps) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
+        const bool r0 = n0 + g < p.N, r1 = n0 + g + 8 < p.N;
+        const uint8_t* b0 = p.b + int64_t(n0 + g) * p.K;
+        const uint8_t* b1 = b0 + int64_t(8) * p.K;
 #pragma unroll
         for (int i = 0; i < kRowsSteps; ++i) {
             const int k = (s0 + i * warps) * 64 + tig * 16;
@@ -229,6 +226,49 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const Int8Params p) {
                 if (r1) w1[i] = __ldg(reinterpret_cast<const uint4*>(b1 + k));
             }
         }
+    }
+    __device__ __forceinline__ void multiply(int* acc, int i, uint4 x) const {
+        mma_s8(acc, w0[i].x, w1[i].x, w0[i].y, w1[i].y, x.x, x.y);
+        mma_s8(acc, w0[i].z, w1[i].z, w0[i].w, w1[i].w, x.z, x.w);
+    }
+};
+
+// The warps' sums of 16 channels and NT groups of eight tokens, added and stored: thread = (token, channel), so that 16
+// consecutive threads write 16 consecutive channels.  red: [warps][NT][16][8]
+template <int NT>
+__device__ __forceinline__ void rows_finish(const Int8Params& p, int (&acc)[NT][4], int* red, const float* a_s, int n0) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, tig = lane & 3;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        int* d = red + (warp * NT + j) * 128;
+        *reinterpret_cast<int2*>(d + g * 8 + tig * 2) = make_int2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<int2*>(d + (g + 8) * 8 + tig * 2) = make_int2(acc[j][2], acc[j][3]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 128; i += blockDim.x) {
+        const int m = i >> 4, ch = i & 15;
+        if (m >= p.M || n0 + ch >= p.N) continue;
+        const int* d = red + (m >> 3) * 128 + ch * 8 + (m & 7);
+        int v = 0;
+        for (int w = 0; w < warps; ++w) v += d[w * NT * 128];
+        store_one(p, int64_t(m) * p.N + n0 + ch, __int2float_rn(v) * a_s[m] * p.b_s[n0 + ch]);
+    }
+}
+
+template <int NT>
+__global__ void __launch_bounds__(512) int8_rows_kernel(const Int8Params p) {
+    extern __shared__ int red[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int g = lane >> 2, tig = lane & 3;
+    const int n0 = blockIdx.x * 16;
+    const int steps = (p.K + 63) >> 6;
+    int acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0;
+    bool waited = false;
+    for (int s0 = warp; s0 < steps; s0 += warps * kRowsSteps) {
+        RowWeights w;
+        w.load(p, n0, s0, warps);
         if (!waited) { grid_wait(); waited = true; }
 #pragma unroll
         for (int i = 0; i < kRowsSteps; ++i) {
@@ -237,28 +277,74 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const Int8Params p) {
             for (int j = 0; j < NT; ++j) {
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (k < p.K && j * 8 + g < p.M) x = *reinterpret_cast<const uint4*>(p.a + int64_t(j * 8 + g) * p.K + k);
-                mma_s8(acc[j], w0[i].x, w1[i].x, w0[i].y, w1[i].y, x.x, x.y);
-                mma_s8(acc[j], w0[i].z, w1[i].z, w0[i].w, w1[i].w, x.z, x.w);
+                w.multiply(acc[j], i, x);
             }
         }
     }
     if (!waited) grid_wait();
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        int* d = red + (warp * NT + j) * 128;
-        *reinterpret_cast<int2*>(d + g * 8 + tig * 2) = make_int2(acc[j][0], acc[j][1]);
-        *reinterpret_cast<int2*>(d + (g + 8) * 8 + tig * 2) = make_int2(acc[j][2], acc[j][3]);
-    }
+    rows_finish<NT>(p, acc, red, p.a_s, n0);
+}
+
+// One token with the quantiser inside: every CTA makes the token's codes itself (from L2, while its weights are on their way).
+// As long as all CTAs run at once that costs about what the kernel in front does, and the second launch is saved: one token
+// through 4096 x 4096 takes 8.3 us a call instead of 8.9 (6.9 us on the GPU, 6.2 in two kernels), through 1024 x 1024 3.5 us on the
+// GPU.  With more tokens or channels the repeated work is longer than the launch (6 x 8192 x 2048: 14 us, 8 in two kernels).
+// The arithmetic is that of token_quant_kernel; CTA 0 leaves codes and scale in the workspaces.
+constexpr int kFusedMaxK = 16384;
+
+template <typename T, bool SMOOTH>
+__global__ void __launch_bounds__(512) int8_one_token_kernel(const Int8Params p, const TokenParams tok) {
+    extern __shared__ int red[];                     // [warps][16][8] sums, then the codes of the token
+    __shared__ int amax;
+    constexpr int ES = sizeof(T);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
+    const int n0 = blockIdx.x * 16, steps = (p.K + 63) >> 6;
+    uint8_t* codes = reinterpret_cast<uint8_t*>(red + warps * 128);
+    RowWeights w;
+    w.load(p, n0, warp, warps);
+    if (t == 0) amax = 0;
     __syncthreads();
-    // thread = (token, channel): 16 consecutive threads write 16 consecutive channels
-    for (int i = threadIdx.x; i < NT * 128; i += blockDim.x) {
-        const int m = i >> 4, ch = i & 15;
-        if (m >= p.M || n0 + ch >= p.N) continue;
-        const int* d = red + (m >> 3) * 128 + ch * 8 + (m & 7);
-        int v = 0;
-        for (int w = 0; w < warps; ++w) v += d[w * NT * 128];
-        store_one(p, int64_t(m) * p.N + n0 + ch, __int2float_rn(v) * p.a_s[m] * p.b_s[n0 + ch]);
+    auto element8 = [&](int c, float2* e) {
+        Vec8<T> v;
+        v.load(tok.x + int64_t(c) * ES);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = v.get(i);
+        if constexpr (SMOOTH) smooth8(tok.smooth + c, e);
+    };
+    float a = 0.f;
+    for (int c = t * 8; c < p.K; c += blockDim.x * 8) {
+        float2 e[4];
+        element8(c, e);
+        a = max_nan(a, amax_pairs(e));
     }
+    // of numbers without a sign the bits are in the order of the values, a NaN's above infinity's
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(a) & 0x7fffffffu);
+    if (lane == 0) atomicMax(&amax, int(bits));
+    __syncthreads();
+    const Divisor d(code_scale<CODES_INT8>(__int_as_float(amax)));
+    for (int c = t * 8; c < p.K; c += blockDim.x * 8) {
+        float2 e[4];
+        element8(c, e);
+        const uint2 q = encode8<CODES_INT8>(e, d);
+        *reinterpret_cast<uint2*>(codes + c) = q;
+        if (blockIdx.x == 0) *reinterpret_cast<uint2*>(tok.q + c) = q;
+    }
+    if (blockIdx.x == 0 && t == 0) tok.s[0] = d.s;
+    __syncthreads();
+    int acc[1][4] = {{0, 0, 0, 0}};
+    for (int s0 = warp; s0 < steps; s0 += warps * kRowsSteps) {
+        if (s0 != warp) w.load(p, n0, s0, warps);
+#pragma unroll
+        for (int i = 0; i < kRowsSteps; ++i) {
+            const int k = (s0 + i * warps) * 64 + (lane & 3) * 16;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (k < p.K && lane < 4) x = *reinterpret_cast<const uint4*>(codes + k);
+            w.multiply(acc[0], i, x);
+        }
+    }
+    __shared__ float scale;
+    if (t == 0) scale = d.s;
+    rows_finish<1>(p, acc, red, &scale, n0);         // its barrier is between
 }
 
 // The tensor-core kernels: 128 x TN tiles of c, k in stages of 128 bytes brought in by TMA, int32 sums in
@@ -856,6 +942,9 @@ int int8_check(const char* what, int64_t M, int64_t N, int64_t K, int out_dtype)
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// warps that share k in the kernels for few tokens: as many as have all their weights in flight at once, at most 16
+int rows_warps(int64_t K) { return int(std::max<int64_t>(2, std::min<int64_t>(16, ceil_div(ceil_div(K, 64), kRowsSteps)))); }
+
 // How many clusters of s CTAs of the split kernel run at once on the current device (asked once per device, tile and s): where
 // there are more of them a second wave doubles the time.
 template <int TN>
@@ -893,8 +982,7 @@ int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
     const int64_t es = p.out_dtype == LH_F32 ? 4 : 2;
     p.wide = p.N % 4 == 0 && aligned(p.b_s, 16);
     if (p.M <= 16) {
-        const int steps = (p.K + 63) / 64;
-        const int warps = std::max(2, std::min(16, (steps + kRowsSteps - 1) / kRowsSteps));
+        const int warps = rows_warps(p.K);
         const unsigned grid = unsigned(ceil_div(p.N, 16));
         if (p.M <= 8) return launch<int8_rows_kernel<1>>("int8_rows_kernel", grid, 32u * warps, size_t(warps) * 512, 1, dependent, stream, p);
         return launch<int8_rows_kernel<2>>("int8_rows_kernel", grid, 32u * warps, size_t(warps) * 1024, 1, dependent, stream, p);
@@ -1020,6 +1108,25 @@ int int8_linear(const void* x, const float* smooth, int dtype, const void* b, co
     if (M == 0) return LH_OK;
     if (!b || !b_s || !c) return fail_arg("int8_linear: NULL pointer");
     if (!aligned(b, 16) || !aligned(c, 16)) return fail_arg("int8_linear: pointers must be 16-byte aligned");
+    if (M == 1 && K <= kFusedMaxK && N <= 32 * int64_t(sm_count())) {      // two CTAs of 16 channels per SM
+        Int8Params p{};
+        p.b = static_cast<const uint8_t*>(b); p.b_s = b_s; p.c = static_cast<uint8_t*>(c);
+        p.M = M; p.N = int(N); p.K = int(K); p.out_dtype = out_dtype;
+        TokenParams t{};
+        t.x = static_cast<const uint8_t*>(x); t.smooth = smooth; t.M = M; t.K = int(K); t.q = static_cast<uint8_t*>(q); t.s = s;
+        const int warps = rows_warps(K);
+        const size_t smem = size_t(warps) * 512 + size_t(K);
+        const unsigned grid = unsigned(ceil_div(N, 16)), threads = 32u * warps;
+        const char* what = "int8_one_token_kernel";
+        auto with = [&](auto type) {
+            using T = decltype(type);
+            return smooth ? launch<int8_one_token_kernel<T, true>>(what, grid, threads, smem, 1, false, stream, p, t)
+                          : launch<int8_one_token_kernel<T, false>>(what, grid, threads, smem, 1, false, stream, p, t);
+        };
+        if (dtype == LH_BF16) return with(__nv_bfloat16{});
+        if (dtype == LH_F16) return with(__half{});
+        return with(float{});
+    }
     if (int rc = token_quant_int8(x, smooth, dtype, M, K, q, s, stream)) return rc;
     return int8_gemm(q, b, s, b_s, c, M, N, K, out_dtype, true, stream);
 }

@@ -346,6 +346,31 @@ def test_int8_linear(lead, N, K, dtype, smooth):
     ok()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("N,K,smooth", [(1, 16, False), (33, 80, True), (4096, 4096, False), (4736, 16384, True), (4752, 1024, False), (512, 16400, True), (1111, 2064, False)])
+def test_int8_linear_of_one_token(N, K, smooth, dtype):
+    """One kernel up to two CTAs of 16 channels per SM and 16384 of k, two beyond: the bits of the two calls, also for a token that is
+    zero and for one with a NaN or an infinity (every result is NaN or infinite then)."""
+    from linghe_b200.gemm.int8_gemm import int8_gemm, int8_linear
+    from linghe_b200.quant.token import token_quant_int8
+    _, b, _, sb = gemm_inputs(1, N, K)
+    b, sb = b.to(DEV), (sb / K).to(DEV)
+    sm = torch.exp(rand(3, K)).to(DEV) if smooth else None
+    x = rand(1, 1, K).to(dtype).to(DEV)
+    for fill in (None, 0.0, float("nan"), float("-inf")):
+        if fill == 0.0:
+            x.zero_()
+        elif fill is not None:
+            x[0, K // 2] = fill
+        got = int8_linear(x, b, sb, smooth_scale=sm)
+        q, s = token_quant_int8(x, sm)
+        if fill is None or fill == 0.0:
+            same(got, int8_gemm(q, b, s, sb, out_dtype=dtype).cpu(), "the two calls in one")
+        else:
+            assert torch.isnan(s).all() and not torch.isfinite(got).any()
+    ok()
+
+
 def test_int8_no_rows():
     from linghe_b200.gemm.int8_gemm import int8_gemm, int8_linear
     from linghe_b200.quant.token import token_quant_int8
