@@ -200,7 +200,8 @@ __device__ __forceinline__ void fetch_scales(const Int8Params& p, int n0, int co
 // them in flight at once.  A CTA takes 16 channels, its warps share k in steps of 64; a lane loads 16 bytes of two channels
 // per step straight into the fragments of mma.m16n8k32 (k may be in any order as long as both operands agree, so
 // a lane's 16 consecutive bytes serve as the two 4-byte pieces of two instructions).  Eight tokens fill the n = 8 of
-// the instruction; NT such groups.  The weights are asked for before the wait for the kernel that writes the codes.
+// the instruction; NT such groups.  The weights are asked for before the wait for the kernel that writes the codes.  64 registers,
+// so that two CTAs of 16 warps are on an SM: 1 x 4096 x 4096 4.2 us (4.0 TB/s; 5.5 us with one), 1 x 8192 x 8192 14.7 us (4.6 TB/s).
 constexpr int kRowsSteps = 4;      // steps of a warp in flight
 
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -256,7 +257,7 @@ __device__ __forceinline__ void rows_finish(const Int8Params& p, int (&acc)[NT][
 }
 
 template <int NT>
-__global__ void __launch_bounds__(512) int8_rows_kernel(const Int8Params p) {
+__global__ void __launch_bounds__(512, NT == 1 ? 2 : 1) int8_rows_kernel(const Int8Params p) {
     extern __shared__ int red[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int g = lane >> 2, tig = lane & 3;
@@ -287,13 +288,13 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const Int8Params p) {
 
 // One token with the quantiser inside: every CTA makes the token's codes itself (from L2, while its weights are on their way).
 // As long as all CTAs run at once that costs about what the kernel in front does, and the second launch is saved: one token
-// through 4096 x 4096 takes 8.3 us a call instead of 8.9 (6.9 us on the GPU, 6.2 in two kernels), through 1024 x 1024 3.5 us on the
-// GPU.  With more tokens or channels the repeated work is longer than the launch (6 x 8192 x 2048: 14 us, 8 in two kernels).
+// through 4096 x 4096 takes 5.5 us on the GPU either way and 0.5 us less a call, through 1024 x 1024 3.8 us.  With more
+// tokens or channels the repeated work is longer than the launch (6 x 8192 x 2048: 14 us, 5.5 in two kernels).
 // The arithmetic is that of token_quant_kernel; CTA 0 leaves codes and scale in the workspaces.
 constexpr int kFusedMaxK = 16384;
 
 template <typename T, bool SMOOTH>
-__global__ void __launch_bounds__(512) int8_one_token_kernel(const Int8Params p, const TokenParams tok) {
+__global__ void __launch_bounds__(512, 2) int8_one_token_kernel(const Int8Params p, const TokenParams tok) {
     extern __shared__ int red[];                     // [warps][16][8] sums, then the codes of the token
     __shared__ int amax;
     constexpr int ES = sizeof(T);
@@ -420,8 +421,9 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-// Large products: one persistent CTA per SM walks tiles (column tile fastest); warp 0 TMA, warp 1 MMA, warps 2-9
-// read the sums of the tile before out of the other tensor-memory buffer, scale and store them.
+// Products of many tiles and little k: one persistent CTA per SM walks tiles (column tile fastest); warp 0 TMA, warp 1 MMA,
+// warps 2-9 read the sums of the tile before out of the other tensor-memory buffer, scale and store them.  Twice as many CTAs
+// store as in the kernel for pairs of SMs below, which is ahead otherwise (4096 x 8192 x 512: 30 us, 39 there).
 template <int TN>
 struct BigTile {
     static constexpr int STAGE = I_ATILE + TN * IKB;
@@ -536,8 +538,9 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 
 // The largest products: two CTAs of a cluster (a pair of SMs) share a 256 x 256 tile, tcgen05.mma.cta_group::2.  Each
 // brings in its 128 rows of a and its 128 rows of b, half of what the pair multiplies, so an SM takes 32 KB per 128 bytes of k
-// where the 128 x 256 tile above takes 48: that kernel waits for L2 (96 bytes per cycle and SM at the full rate of the tensor
-// cores), this one needs 64.  The leader (rank 0) issues for both; full[] counts in the leader's shared memory what both
+// for 128 x 256 sums; a CTA alone takes 48, 96 bytes per cycle at the full rate of the tensor cores, more than L2 gives (8192 x
+// 8192 x 4096: 201 us against 178, 8192^3: 485 against 364).  From about 4096 of k on the power limit bounds it: 0.40 us per 128
+// of k where a short run takes 0.26; below 1024 of k the stores do, about 5 us per tile.  The leader (rank 0) issues for both; full[] counts in the leader's shared memory what both
 // bring, commits arrive in both CTAs, both read their half of the sums.
 struct PairTile {
     static constexpr int TN = 256, TM = 256;
@@ -942,8 +945,13 @@ int int8_check(const char* what, int64_t M, int64_t N, int64_t K, int out_dtype)
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// warps that share k in the kernels for few tokens: as many as have all their weights in flight at once, at most 16
-int rows_warps(int64_t K) { return int(std::max<int64_t>(2, std::min<int64_t>(16, ceil_div(ceil_div(K, 64), kRowsSteps)))); }
+// Warps that share k in the kernels for few tokens: as many as have all their weights in flight at once, at most 16; 8 where there
+// are more CTAs of 16 channels than two per SM, so that the next ones load while these finish (1 x 8192 x 8192 14.7 us, 16.6
+// with 16 warps; 4 x 4096 x 14336 17.1 and 14.5).
+int rows_warps(int64_t N, int64_t K) {
+    const int64_t most = N > 32 * int64_t(sm_count()) ? 8 : 16;
+    return int(std::max<int64_t>(2, std::min<int64_t>(most, ceil_div(ceil_div(K, 64), kRowsSteps))));
+}
 
 // How many clusters of s CTAs of the split kernel run at once on the current device (asked once per device, tile and s): where
 // there are more of them a second wave doubles the time.
@@ -982,7 +990,7 @@ int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
     const int64_t es = p.out_dtype == LH_F32 ? 4 : 2;
     p.wide = p.N % 4 == 0 && aligned(p.b_s, 16);
     if (p.M <= 16) {
-        const int warps = rows_warps(p.K);
+        const int warps = rows_warps(p.N, p.K);
         const unsigned grid = unsigned(ceil_div(p.N, 16));
         if (p.M <= 8) return launch<int8_rows_kernel<1>>("int8_rows_kernel", grid, 32u * warps, size_t(warps) * 512, 1, dependent, stream, p);
         return launch<int8_rows_kernel<2>>("int8_rows_kernel", grid, 32u * warps, size_t(warps) * 1024, 1, dependent, stream, p);
@@ -1114,7 +1122,7 @@ int int8_linear(const void* x, const float* smooth, int dtype, const void* b, co
         p.M = M; p.N = int(N); p.K = int(K); p.out_dtype = out_dtype;
         TokenParams t{};
         t.x = static_cast<const uint8_t*>(x); t.smooth = smooth; t.M = M; t.K = int(K); t.q = static_cast<uint8_t*>(q); t.s = s;
-        const int warps = rows_warps(K);
+        const int warps = rows_warps(N, K);
         const size_t smem = size_t(warps) * 512 + size_t(K);
         const unsigned grid = unsigned(ceil_div(N, 16)), threads = 32u * warps;
         const char* what = "int8_one_token_kernel";

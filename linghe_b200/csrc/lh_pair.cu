@@ -64,9 +64,9 @@ enum : int { GATE_NONE = 0, GATE_ROW = 1, GATE_GROUPS = 2, GATE_EACH = 3 };   //
 // One CTA per row, a thread 32 consecutive bytes of it in registers, every load of the row asked for at once: with
 // 64 registers 1024 threads are resident, so four rows of 4096 are on their way to an SM while others are normalised
 // or stored.  Coefficients (the same for every row) come from L1 and L2: with the row where registers allow it (16-bit
-// types without checkpoints, 85 us; 88 where they are fetched when wanted), behind the sums elsewhere (with int8
+// types without checkpoints, 87 us; 88 where they are fetched when wanted), behind the sums elsewhere (with int8
 // checkpoints 122 us, 155 - 175 the other way).
-// Measured at 16384 x 4096, bf16: 85 us (97 % of the measured copy bandwidth).  A persistent walk fed by bulk copies through a
+// Measured at 16384 x 4096, bf16: 87 us (94 % of the measured copy bandwidth), 92 with a gate.  A persistent walk fed by bulk copies through a
 // shared-memory ring took 92 - 102 us whatever its depth, order of rows, rows per step or cache hints, and 4.2 us
 // instead of 3.2 for 16 rows.
 
@@ -230,7 +230,8 @@ __device__ __forceinline__ float2 cta_sum2(float a, float b, float* buf) {
 template <typename T, int CK, int GATE>
 __global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const PairParams p) {
     extern __shared__ __align__(128) uint8_t ring[];
-    constexpr int NB = kPairMaxN / 128, SC = 2 * NB + 2, DEPTH = kPairMaxStages + 2;
+    constexpr int NB = kPairMaxN / 128, SC = 2 * NB + 2;
+    constexpr int DEPTH = kPairMaxStages + 3;      // behind the barrier of row i: row i in pass 3 up to row i + S + 2 on its way
     __shared__ uint64_t full[kPairMaxStages];
     __shared__ float sums[2][32];
     __shared__ float scal[DEPTH][SC];        // scales of o, of h, 1/rms of o, of h

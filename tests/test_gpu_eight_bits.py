@@ -141,6 +141,15 @@ def test_pair_backward_gate_groups(lead):
     pair_backward_case(lead, 2048, torch.float32, "sample", None)
 
 
+# many rows to a CTA, so that every slot of its rings is used again several times
+@pytest.mark.parametrize("kind", [None, *KINDS], ids=name)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=name)
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("lead,n", [((12000, 5), 128), ((1400, 5), 1408), ((301, 5), 5120), ((300, 4), 8192)])
+def test_pair_backward_long_walks(lead, n, dtype, gate, kind):
+    pair_backward_case(lead, n, dtype, gate, kind)
+
+
 def test_pair_no_rows():
     from linghe_b200.utils.norm import rms_norm_pair_backward, rms_norm_pair_forward
     x = torch.empty((0, 256), dtype=torch.bfloat16, device=DEV)
@@ -175,7 +184,7 @@ def test_pair_values_that_are_not_finite():
 @pytest.mark.parametrize("weight", [None, torch.float32, torch.bfloat16], ids=["none", "f32", "bf16"])
 @pytest.mark.parametrize("kind", KINDS, ids=name)
 @pytest.mark.parametrize("dtype", TYPES, ids=name)
-@pytest.mark.parametrize("M,n", [(1, 128), (3, 256), (77, 512), (130, 1408), (65, 4096), (9, 8192), (5, 14336)])
+@pytest.mark.parametrize("M,n", [(1, 128), (3, 256), (77, 512), (130, 1408), (65, 4096), (9, 8192), (5, 14336), (5001, 1408), (4800, 384)])
 def test_silu_checkpoint(M, n, dtype, kind, weight):
     from linghe_b200.utils.silu import silu_and_checkpoint_backward, silu_and_checkpoint_forward
     x, g = rand(1, M, 2 * n, scale=3).to(dtype), rand(2, M, n).to(dtype)
@@ -287,7 +296,8 @@ def gemm_inputs(M, N, K, seed=1):
 # one to sixteen tokens, then every kernel and its ragged edges: rows, columns, k within a stage and past it
 GEMMS = [(1, 16, 16), (1, 4096, 4096), (3, 17, 80), (8, 1000, 2064), (9, 256, 512), (16, 33, 1040),
          (17, 40, 16), (17, 4096, 4096), (64, 512, 8192), (100, 1111, 528), (128, 64, 128), (129, 300, 2048), (200, 4096, 1024), (257, 63, 4096),
-         (640, 4096, 272), (1000, 1111, 2064), (2048, 2500, 384), (1500, 4352, 144), (3000, 5000, 16)]
+         (640, 4096, 272), (1000, 1111, 2064), (2048, 2500, 384), (1500, 4352, 144), (3000, 5000, 16),
+         (4100, 8200, 144), (4100, 4099, 400), (2100, 16400, 528), (6000, 6016, 1040)]     # many tiles to a CTA
 
 
 @pytest.mark.parametrize("out_dtype", TYPES, ids=name)
