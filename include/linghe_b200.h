@@ -95,7 +95,7 @@ int lh_selftest_wait_timeout(int polls, void* stream);
  *                                narrower ones the TMA ring (default 1536) */
 int lh_tuning(const char* key, int value);
 
-/* Scratch bytes needed by the entry point named `what` ("rmsnorm_bwd",
+/* Scratch bytes needed by the entry point named `what` ("rmsnorm_bwd", "rmsnorm_pair_bwd",
  * "batch_silu_bwd") for the given sizes; 0 if it needs none, <0 if unknown. */
 int64_t lh_scratch_bytes(const char* what, int64_t rows, int64_t cols);
 
