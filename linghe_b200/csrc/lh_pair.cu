@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kPairMaxN = 8192;
 constexpr int kPairMaxThreads = kPairMaxN / 16;
+constexpr int kPairOneMaxN = 5120;          // backward, rows of one vector a thread: up to 640 threads, 96 registers each
 constexpr int kPairThreadsPerSm = 512;     // backward, 128 registers a thread
 constexpr int kPairMaxStages = 4;
 constexpr int kPairSmem = 227 * 1024;      // shared memory of an SM that CTAs can ask for
@@ -206,16 +207,19 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Sums over the CTA of two values.  buf: a place for each of 16 warps and value, those of absent warps zeroed.
+// Sums over the CTA of two values.  buf: a place for each of W (16 or 32) warps and value, those of absent warps zeroed.
+template <int W>
 __device__ __forceinline__ float2 cta_sum2(float a, float b, float* buf) {
     const bool up = (threadIdx.x & 16) != 0;          // the halves of a warp take a value each after the first exchange
     float v = up ? b : a;
     v += __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    if ((threadIdx.x & 15) == 0) buf[(threadIdx.x & 16) + (threadIdx.x >> 5)] = v;
+    if ((threadIdx.x & 15) == 0) buf[(threadIdx.x & 16) * (W / 16) + (threadIdx.x >> 5)] = v;
     __syncthreads();
-    v = buf[threadIdx.x & 31];
+    const float* mine = buf + (threadIdx.x & 16) * (W / 16) + (threadIdx.x & 15);
+    v = mine[0];
+    if (W == 32) v += mine[16];
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     const float o = __shfl_xor_sync(0xffffffffu, v, 16);
@@ -225,18 +229,18 @@ __device__ __forceinline__ float2 cta_sum2(float a, float b, float* buf) {
 // A row passes three times through the registers: (1) sum t * hn, (2) dx, the sums over rows, u and sum u * on,
 // (3) do.  The two sums of a row are joined with its neighbours': between two barriers a CTA does (3) of row i, (2) of
 // row i + 1 and (1) of row i + 2, and the barrier exchanges the sums of the latter two.  That is one barrier and one
-// reduction's latency per row, with 16 warps on an SM (128 registers a thread) to hide it.  Rows come in by bulk copies,
+// reduction's latency per row, with 16 to 20 warps on an SM to hide it.  Rows come in by bulk copies,
 // their 1/rms and the scales of their codes by 4-byte copies two rows further ahead.
-template <typename T, int CK, int GATE>
-__global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const PairParams p) {
+template <typename T, int CK, int GATE, int V>
+__global__ void __launch_bounds__(V == 1 ? kPairOneMaxN / 8 : kPairMaxThreads, 1) pair_bwd_kernel(const PairParams p) {
     extern __shared__ __align__(128) uint8_t ring[];
     constexpr int NB = kPairMaxN / 128, SC = 2 * NB + 2;
     constexpr int DEPTH = kPairMaxStages + 3;      // behind the barrier of row i: row i in pass 3 up to row i + S + 2 on its way
     __shared__ uint64_t full[kPairMaxStages];
-    __shared__ float sums[2][32];
+    constexpr int W = V == 1 ? 32 : 16;       // warps of a CTA, at most
+    __shared__ float sums[2][2 * W];
     __shared__ float scal[DEPTH][SC];        // scales of o, of h, 1/rms of o, of h
     constexpr bool GROUPS = GATE == GATE_GROUPS, EACH = GATE == GATE_EACH;
-    constexpr int V = 2;           // vectors of a thread in a row; one (64 registers, twice the warps) measured a quarter slower
     constexpr int ES = sizeof(T), CS = CK == CODES_NONE ? ES : 1;   // bytes of an element of dy / of o and h
     const int t = threadIdx.x, nt = blockDim.x, S = p.stages, nb = p.n >> 7;
     const uint32_t row_bytes = uint32_t(p.n) * ES, code_bytes = uint32_t(p.n) * CS;
@@ -301,7 +305,7 @@ __global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const Pair
         for (int s = 0; s < S && begin + s < end; ++s) fetch(s);
     }
     for (int i = 0; i < S + 2; ++i) fetch_scalars();
-    if (t < 32) sums[0][t] = sums[1][t] = 0.f;
+    if (t < 2 * W) sums[0][t] = sums[1][t] = 0.f;
 
     int col[V];
     bool live[V];
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const Pair
         int sl = 0, sc = 0, par = 0;                 // stage, slot of the scalars of the row of pass 2
         uint32_t ph = 0;
         const uint8_t* st = ring;
-        float2 sum = cta_sum2(pass1(st, scal[0]), 0.f, sums[par]);
+        float2 sum = cta_sum2<W>(pass1(st, scal[0]), 0.f, sums[par]);
         par ^= 1;
         float part2 = pass2(st, scal[0], sum.x * p.inv_n, u, dx_row);
         while (true) {
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const Pair
                 part1 = pass1(st, scal[sc]);
             }
             copies_wait<1>();
-            sum = cta_sum2(part1, part2, sums[par]);
+            sum = cta_sum2<W>(part1, part2, sums[par]);
             par ^= 1;
             // behind that barrier every thread has read the stage of the row whose pass 2 came before it
             if (t == 0 && at2.j + S < end) fetch(done);
@@ -505,11 +509,11 @@ __global__ void __launch_bounds__(kPairMaxThreads, 1) pair_bwd_kernel(const Pair
         int sc = 0;
         uint32_t ph = 0;
         while (true) {
-            float2 sum = cta_sum2(pass1(ring, scal[sc]), 0.f, sums[0]);
+            float2 sum = cta_sum2<W>(pass1(ring, scal[sc]), 0.f, sums[0]);
             const float part = pass2(ring, scal[sc], sum.x * p.inv_n, u, dx_row);
             fetch_scalars();
             copies_wait<0>();
-            sum = cta_sum2(part, 0.f, sums[1]);
+            sum = cta_sum2<W>(part, 0.f, sums[1]);
             if (t == 0 && at2.j + 1 < end) fetch(0);
             pass3(scal[sc], sum.x * p.inv_n, u, do_row);
             if (at2.j + 1 == end) break;
@@ -599,10 +603,15 @@ __global__ void __launch_bounds__(256) pair_reduce_kernel(const float* part, int
     }
 }
 
-// The backward kernel wants 128 registers a thread, so 512 threads fill an SM: CTAs of rows of up to 4096 columns share it, wider
-// ones are alone on it.  (Two CTAs of 320 threads with 96 registers each spill: 86 us instead of 73 at 5005 x 5120, int8.)
-int pair_threads(int64_t n) { return int((n / 16 + 31) / 32 * 32); }
-int pair_per_sm(int64_t n) { return std::max(1, std::min(32, kPairThreadsPerSm / pair_threads(n))); }
+// With two vectors of eight elements a thread the backward kernel wants 128 registers, so 512 threads fill an SM: CTAs of rows of
+// up to 4096 columns share it, wider ones are alone on it and leave up to seven of 16 warps out.  16-bit rows of 4097 to 5120 columns
+// therefore take one vector a thread, 17 to 20 warps of 96 registers: fp16 at 5005 x 5120 75 -> 61 us, from int8 73 -> 66, with
+// a gate per sample 86 -> 75; 8192 x 4224 109 -> 91.  Up to 6144 columns that is 80 registers, which spill (5005 x 5120 67 and
+// 87 us); float32 rows gain nothing from int8 (106 -> 109) and 1 to 7 % without codes; one vector a thread with 64 registers
+// and 32 warps is a quarter slower at 4096 columns.
+template <typename T>
+int pair_vectors(int64_t n) { return sizeof(T) == 2 && n > 4096 && n <= kPairOneMaxN ? 1 : 2; }
+int pair_per_sm(int64_t n) { return std::max(1, std::min(32, kPairThreadsPerSm / int((n / 16 + 31) / 32 * 32))); }
 // Stages of `bytes` each, with `fixed` bytes beside them; fewer CTAs per SM where there is no room for two stages
 void pair_shape(int64_t bytes, int64_t fixed, int& per_sm, int& stages) {
     while (true) {
@@ -638,27 +647,32 @@ int64_t pair_bwd_grid(int64_t M, int64_t n) {
 
 template <typename T>
 int pair_bwd_typed(PairParams& p, int ck, float* dpost, float* dpre, cudaStream_t stream) {
-    const int nt = pair_threads(p.n);
+    const int vectors = pair_vectors<T>(p.n), nt = int((p.n / (8 * vectors) + 31) / 32 * 32);
     const int64_t code = ck == CODES_NONE ? int64_t(sizeof(T)) : 1;
     const bool each = p.gate && p.G == p.M && p.M > 1, groups = p.gate && p.G > 1 && !each;
     const int64_t bytes = p.n * (int64_t(sizeof(T)) * (1 + (p.dh ? 1 : 0) + (each ? 1 : 0)) + 2 * code);
     int per_sm = pair_per_sm(p.n);
-    const int64_t fixed = groups ? int64_t(nt) * 64 : 0;
+    const int64_t fixed = groups ? int64_t(nt) * 32 * vectors : 0;
     pair_shape(bytes, fixed, per_sm, p.stages);
     const int64_t grid = std::min(pair_bwd_grid(p.M, p.n), int64_t(sm_count()) * per_sm);
     const int64_t smem = bytes * p.stages + fixed;
     const char* what = "pair_bwd_kernel";
     int rc;
-    auto with = [&](auto codes) {
-        constexpr int CK = decltype(codes)::value;
-        if (!p.gate) return pair_launch<pair_bwd_kernel<T, CK, GATE_NONE>>(grid, nt, smem, p, what, stream);
-        if (p.G == 1) return pair_launch<pair_bwd_kernel<T, CK, GATE_ROW>>(grid, nt, smem, p, what, stream);
-        return each ? pair_launch<pair_bwd_kernel<T, CK, GATE_EACH>>(grid, nt, smem, p, what, stream)
-                    : pair_launch<pair_bwd_kernel<T, CK, GATE_GROUPS>>(grid, nt, smem, p, what, stream);
+    auto with = [&](auto codes, auto width) {
+        constexpr int CK = decltype(codes)::value, V = decltype(width)::value;
+        if (!p.gate) return pair_launch<pair_bwd_kernel<T, CK, GATE_NONE, V>>(grid, nt, smem, p, what, stream);
+        if (p.G == 1) return pair_launch<pair_bwd_kernel<T, CK, GATE_ROW, V>>(grid, nt, smem, p, what, stream);
+        return each ? pair_launch<pair_bwd_kernel<T, CK, GATE_EACH, V>>(grid, nt, smem, p, what, stream)
+                    : pair_launch<pair_bwd_kernel<T, CK, GATE_GROUPS, V>>(grid, nt, smem, p, what, stream);
     };
-    if (ck == CODES_INT8) rc = with(std::integral_constant<int, CODES_INT8>{});
-    else if (ck == CODES_E4M3) rc = with(std::integral_constant<int, CODES_E4M3>{});
-    else rc = with(std::integral_constant<int, CODES_NONE>{});
+    auto of = [&](auto codes) {
+        if constexpr (sizeof(T) == 2)
+            if (vectors == 1) return with(codes, std::integral_constant<int, 1>{});
+        return with(codes, std::integral_constant<int, 2>{});
+    };
+    if (ck == CODES_INT8) rc = of(std::integral_constant<int, CODES_INT8>{});
+    else if (ck == CODES_E4M3) rc = of(std::integral_constant<int, CODES_E4M3>{});
+    else rc = of(std::integral_constant<int, CODES_NONE>{});
     if (rc) return rc;
     const int64_t looks = groups ? std::min<int64_t>(p.G, grid - 1) : 0;
     cudaLaunchConfig_t cfg{};

@@ -150,6 +150,15 @@ def test_pair_backward_long_walks(lead, n, dtype, gate, kind):
     pair_backward_case(lead, n, dtype, gate, kind)
 
 
+# widths on both sides of where a thread has one vector of a row instead of two; the second ends inside a warp
+@pytest.mark.parametrize("kind", [None, torch.int8], ids=name)
+@pytest.mark.parametrize("dtype", TYPES, ids=name)
+@pytest.mark.parametrize("gate", GATES)
+@pytest.mark.parametrize("n", [4096, 4224, 4992, 5248])
+def test_pair_backward_widths(n, dtype, gate, kind):
+    pair_backward_case((180, 5), n, dtype, gate, kind)
+
+
 def test_pair_no_rows():
     from linghe_b200.utils.norm import rms_norm_pair_backward, rms_norm_pair_forward
     x = torch.empty((0, 256), dtype=torch.bfloat16, device=DEV)
