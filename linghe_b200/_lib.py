@@ -174,6 +174,13 @@ def check_same(ref: torch.Tensor, dtype, shape, **tensors):
         assert t.is_contiguous(), f"{name} must be contiguous"
 
 
+def ready(t):
+    """`t` contiguous and at a 16-byte boundary, copied where it is not: autograd hands over views of any offset, such as
+    the piece of a concatenation's gradient."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def ptr(t):
     """device address of a tensor, 0 for None (a NULL pointer at the C ABI)"""
     return 0 if t is None else t.data_ptr()

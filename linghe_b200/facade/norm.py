@@ -10,6 +10,7 @@ import torch
 
 from torch.autograd.function import once_differentiable
 
+from linghe_b200 import _lib
 from linghe_b200.utils.norm import (rms_norm_pair_backward, rms_norm_pair_forward,
                                     triton_rms_norm_and_block_quant_forward, triton_rms_norm_backward,
                                     triton_rms_norm_forward)
@@ -115,7 +116,7 @@ class RMSNormPair(torch.autograd.Function):
         if grad_y is None:        # the second norm leads nowhere
             grad_y = torch.zeros_like(grad_h)
         dx, do, dpost, dpre, dgate = rms_norm_pair_backward(
-            grad_y.contiguous(), None if grad_h is None else grad_h.contiguous(), o, h, post_weight, pre_weight, rms_post, rms_pre,
+            _lib.ready(grad_y), None if grad_h is None else _lib.ready(grad_h), o, h, post_weight, pre_weight, rms_post, rms_pre,
             gate, ctx.residual_scale, o_scale, h_scale)
         return dx, do, dpost, dpre, dgate, None, None, None
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from linghe_b200 import _lib
 from linghe_b200.utils.silu import (silu_and_checkpoint_backward, silu_and_checkpoint_forward,
                                     triton_batch_weighted_silu_and_block_quant_backward,
                                     triton_batch_weighted_silu_and_block_quant_forward,
@@ -120,7 +121,7 @@ class CheckpointedSilu(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_output):
         x_q, x_scale, weight = ctx.saved_tensors
-        g = grad_output.contiguous().view(-1, grad_output.shape[-1])
+        g = _lib.ready(grad_output).view(-1, grad_output.shape[-1])
         dx, dw = silu_and_checkpoint_backward(g, x_q, x_scale, None if weight is None else weight.reshape(-1))
         return dx.view(ctx.shape), None if dw is None else dw.view(weight.shape), None
 
