@@ -5,7 +5,14 @@ comes, where a kernel may round, how far a float32 evaluation may be from it.
 Bounds.  U = 2^-24 is the largest relative error of one float32 rounding.  A kernel evaluates every expression
 here in at most CHAIN roundings in a row, the sum over a row included (at most 16 terms per thread, then a tree), so a
 term of size |t| is off by at most CHAIN * U * |t|, and a sum by that of the sum of its terms' sizes.  A sum over M
-rows adds at most M more roundings.  Rounding the result to its type adds half a step, eps / 2 of its size."""
+rows adds at most M more roundings (`depth` where the number of additions in a row is known).  Rounding the result to its
+type adds half a step, eps / 2 of its size.
+
+A bound that grows with the number of terms cannot tell a lost row from rounding where the terms have both signs.
+`whole_rows` makes inputs for which every sum over rows is exact in float32 and every row adds to every column with the same
+sign: there a lost, doubled or wrongly scaled row is a wrong number."""
+
+import math
 
 import torch
 
@@ -67,9 +74,16 @@ def norm_of(h, weight, eps):
     return y, CHAIN * U * y.abs(), r
 
 
-def pair_backward(dy, dh, o, h, post, pre, r_post, r_pre, gate, alpha):
-    """All [M, n] in float64 (gate too, expanded; dh and gate may be None).  {name: (value, bound)}: dgate per element."""
-    M = dy.shape[0]
+def row_depth(M, sms=148):
+    """Additions in a row behind a sum over M rows in lh_rmsnorm_pair_bwd: at most ceil(M / sms) rows of a CTA (there are at least
+    as many CTAs as SMs, or one per row) and as many groups of gate rows, then up to 16 CTAs an SM in 32 strands, then the strands."""
+    return 2 * math.ceil(M / sms) + math.ceil(16 * sms / 32) + 32
+
+
+def pair_backward(dy, dh, o, h, post, pre, r_post, r_pre, gate, alpha, depth=None):
+    """All [M, n] in float64 (gate too, expanded; dh and gate may be None).  {name: (value, bound)}: dgate per element.
+    depth: additions in a row behind a sum over rows, M if not given."""
+    M = dy.shape[0] if depth is None else depth
     dy, post, pre = dy.double(), post.double(), pre.double()
     r_post, r_pre = r_post.double()[:, None], r_pre.double()[:, None]
     gate = torch.ones_like(dy) if gate is None else gate.double()
@@ -93,6 +107,39 @@ def pair_backward(dy, dh, o, h, post, pre, r_post, r_pre, gate, alpha):
         "dpre": ((dy * hn).sum(0), rows * (dy * hn).abs().sum(0)),
         "dgate": (dgate, 2 * rows * abs(alpha) * (size_dx * on * post).abs()),
     }
+
+
+def whole_rows(lead, n, gate, with_dh=True, seed=1, device="cpu"):
+    """Inputs of the norm pair's gradient and its results, all float64: (inputs, dx and the sums over rows, the terms of the sums).
+
+    o and h are 1 or 2 in neighbouring columns alike, times a power of two per row (1/rms) and, as codes, per block of 128;
+    dy is +1, -1 in neighbouring columns and pre the same in both, so that the row's sum of dy * pre * h * r_pre is zero and
+    dx = dh + r_pre * dy * pre a whole number of 1 to 10 (without dh: one of -4 to 4, no zero, of one sign in a column).  Terms are multiples of 1/4: dx * on <= 20, with the gate and
+    alpha = 1/2 again at most 20; 60000 rows sum to 1.2e6, 4.8e6 quarters, below 2^24.  dy, weights, gates, o, h and the codes
+    (1 to 8) are exact in every type."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+    rows = math.prod(lead)
+
+    def pick(values, *shape):
+        return torch.tensor(values, dtype=torch.float64, device=device)[torch.randint(len(values), shape, generator=gen, device=device)]
+
+    pairs = lambda t: t.repeat_interleave(2, dim=-1)  # noqa: E731
+    sign = torch.tensor([1.0, -1.0], dtype=torch.float64, device=device).repeat(n // 2)
+    d = {"o": pairs(pick([1, 2], rows, n // 2)), "h": pairs(pick([1, 2], rows, n // 2)), "dy": sign.expand(rows, n),
+         "dh": pick([5, 6], rows, n) if with_dh else None, "post": pick([1, 2], n), "pre": pairs(pick([1, 2], n // 2)),
+         "r_post": pick([0.5, 1], rows), "r_pre": pick([1, 2], rows), "alpha": 0.5,
+         "o_scale": pick([0.25, 0.5, 1], rows, n // 128), "h_scale": pick([0.25, 0.5, 1], rows, n // 128)}
+    shape = {"none": None, "channel": (n,), "sample": (lead[-1], n), "token": (*lead, n)}[gate]
+    d["gate"] = None if shape is None else pick([1, 2], *shape)
+    full = torch.ones((), dtype=torch.float64, device=device) if shape is None else d["gate"].expand(*lead, n).reshape(rows, n)
+    on, hn = d["o"] * d["r_post"][:, None], d["h"] * d["r_pre"][:, None]
+    dx = d["r_pre"][:, None] * d["dy"] * d["pre"] + (d["dh"] if with_dh else 0)
+    terms = {"dpre": d["dy"] * hn, "dpost": d["alpha"] * full * dx * on, "dgate": d["alpha"] * dx * on * d["post"]}
+    sums = {"dx": dx, "dpre": terms["dpre"].sum(0), "dpost": terms["dpost"].sum(0)}
+    if shape is not None:
+        G = d["gate"].numel() // n
+        sums["dgate"] = terms["dgate"].view(rows // G, G, n).sum(0).view(shape)
+    return d, sums, terms
 
 
 def silu_terms(x1):
