@@ -10,12 +10,20 @@ import torch
 from linghe_b200 import _lib
 
 
+def _no_gradient(*tensors):
+    """A gradient that would be lost without a word is refused."""
+    assert not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)), (
+        "the int8 product has no backward pass: call it under torch.no_grad() or on detached tensors")
+
+
 def int8_gemm(a, b, a_s, b_s, out_dtype=torch.bfloat16):
     """c [..., N] = (a @ b.T) * a_s[:, None] * b_s for int8 `a` [..., K] and `b` [N, K], float32 `a_s` (one per row of
-    a) and `b_s` [N].  K is a multiple of 16, at most 131056; out_dtype bf16, fp16 or fp32."""
+    a) and `b_s` [N].  K is a multiple of 16, at most 131056; out_dtype bf16, fp16 or fp32.
+    There is no backward pass: scales that require a gradient are refused unless the call is under torch.no_grad()."""
     host = _lib.host()
     if host is not None:   # the same steps in C++ (host/lh_host.cpp)
         return host.int8_gemm(a, b, a_s, b_s, out_dtype)
+    _no_gradient(a_s, b_s)
     assert out_dtype in _lib._DTYPES, f"unsupported out_dtype {out_dtype}"
     N, K = b.shape
     assert a.dim() >= 1 and a.shape[-1] == K, f"a has {a.shape[-1]} columns, b has {K}"
@@ -34,12 +42,14 @@ def int8_linear(x, w, w_s, smooth_scale=None, out_dtype=None):
     [N, K] with one float32 scale `w_s` [N] per output channel: `token_quant_int8` and `int8_gemm` in one call.
 
     `smooth_scale` (float32 [K]): x is divided by it before it is quantised; the weights hold the product with it.
-    The result has `out_dtype`, that of x by default."""
+    The result has `out_dtype`, that of x by default.  There is no backward pass: an x, w_s or smooth_scale that requires a
+    gradient is refused unless the call is under torch.no_grad()."""
     host = _lib.host()
     if host is not None:
         return host.int8_linear(x, w, w_s, smooth_scale, out_dtype)
     if out_dtype is None:
         out_dtype = x.dtype
+    _no_gradient(x, w_s, smooth_scale)
     assert out_dtype in _lib._DTYPES, f"unsupported out_dtype {out_dtype}"
     N, K = w.shape
     assert x.dim() >= 1 and x.shape[-1] == K, f"x has {x.shape[-1]} columns, w has {K}"

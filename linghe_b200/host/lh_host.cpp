@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -340,6 +341,13 @@ std::tuple<at::Tensor, at::Tensor> token_quant_int8(const at::Tensor& x, const O
     return {*out, *scale};
 }
 
+// a gradient that would be lost without a word is refused
+void no_gradient(std::initializer_list<const at::Tensor*> tensors) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const at::Tensor* t : tensors)
+        LH_NEED(t == nullptr || !t->requires_grad(), "the int8 product has no backward pass: call it under torch.no_grad() or on detached tensors");
+}
+
 int out_code(at::ScalarType t) {
     switch (t) {
         case at::kBFloat16: return LH_BF16;
@@ -350,6 +358,7 @@ int out_code(at::ScalarType t) {
 }
 
 at::Tensor int8_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& a_s, const at::Tensor& b_s, at::ScalarType out_dtype) {
+    no_gradient({&a_s, &b_s});
     const int od = out_code(out_dtype);
     LH_NEED(b.dim() == 2 && a.dim() >= 1 && a.size(-1) == b.size(1), "a and b must have the same number of columns");
     const int64_t N = b.size(0), K = b.size(1);
@@ -368,6 +377,7 @@ at::Tensor int8_gemm(const at::Tensor& a, const at::Tensor& b, const at::Tensor&
 }
 
 at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_s, const OptT& smooth, const std::optional<at::ScalarType>& out_dtype) {
+    no_gradient({&x, &w_s, smooth.has_value() ? &*smooth : nullptr});
     const at::ScalarType type = out_dtype.has_value() ? *out_dtype : x.scalar_type();
     const int od = out_code(type), dt = dtype_code(x);
     LH_NEED(w.dim() == 2 && x.dim() >= 1 && x.size(-1) == w.size(1), "x and w must have the same number of columns");
