@@ -258,7 +258,7 @@ __device__ __forceinline__ void rows_finish(const Int8Params& p, int (&acc)[NT][
 
 template <int NT>
 __global__ void __launch_bounds__(512, NT == 1 ? 2 : 1) int8_rows_kernel(const Int8Params p) {
-    extern __shared__ int red[];
+    extern __shared__ __align__(16) int red[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int g = lane >> 2, tig = lane & 3;
     const int n0 = blockIdx.x * 16;
@@ -295,7 +295,7 @@ constexpr int kFusedMaxK = 16384;
 
 template <typename T, bool SMOOTH>
 __global__ void __launch_bounds__(512, 2) int8_one_token_kernel(const Int8Params p, const TokenParams tok) {
-    extern __shared__ int red[];                     // [warps][16][8] sums, then the codes of the token
+    extern __shared__ __align__(16) int red[];       // [warps][16][8] sums, then the codes of the token
     __shared__ int amax;
     constexpr int ES = sizeof(T);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, warps = blockDim.x >> 5;
