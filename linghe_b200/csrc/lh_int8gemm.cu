@@ -421,6 +421,21 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
+// A wait that gave up ends the loop of its warp. What the two issuing warps have issued may still be in flight then, to shared
+// memory and tensor memory that other CTAs own once this one is gone: both leave their loops only when it is complete, or after
+// another time limit. s, ph: the stage a warp would use next and the parity of its pass over the ring; first: its first pass.
+template <int STAGES>
+__device__ __forceinline__ void drain_copies(uint64_t* full, int s, uint32_t ph, bool first) {
+    for (int i = 0; i < STAGES; ++i)
+        if (i < s || !first) mbar_wait_inline(&full[i], i < s ? ph : ph ^ 1u, DEVERR_FULL_WAIT);
+}
+// the commit of the last stage stands for all MMAs before it
+template <int STAGES>
+__device__ __forceinline__ void drain_mmas(uint64_t* empty, int s, uint32_t ph, bool first) {
+    if (s > 0) mbar_wait_inline(&empty[s - 1], ph, DEVERR_EMPTY_WAIT);
+    else if (!first) mbar_wait_inline(&empty[STAGES - 1], ph ^ 1u, DEVERR_EMPTY_WAIT);
+}
+
 // Products of many tiles and little k: one persistent CTA per SM walks tiles (column tile fastest); warp 0 TMA, warp 1 MMA,
 // warps 2-9 read the sums of the tile before out of the other tensor-memory buffer, scale and store them.  Twice as many CTAs
 // store as in the kernel for pairs of SMs below, which is ahead otherwise (4096 x 8192 x 512: 30 us, 39 there).
@@ -485,10 +500,11 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (++s == C::STAGES) { s = 0; ph ^= 1u; first = false; }
             }
         }
+        drain_copies<C::STAGES>(full, s, ph, first);
     } else if (warp == 1) {
         int s = 0;
         uint32_t ph = 0, n = 0;                       // n: tiles so far
-        bool ok = true;
+        bool first = true, ok = true;
         for (int64_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
             const uint32_t buf = n & 1u;
             if (n >= 2) ok = __all_sync(0xffffffffu, mbar_wait_inline(&acc_empty[buf], ((n >> 1) & 1u) ^ 1u, DEVERR_PART_WAIT));
@@ -505,9 +521,10 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     umma_commit(&empty[s]);
                     if (kb == kblocks - 1) umma_commit(&acc_full[buf]);
                 }
-                if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+                if (++s == C::STAGES) { s = 0; ph ^= 1u; first = false; }
             }
         }
+        drain_mmas<C::STAGES>(empty, s, ph, first);
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         EpiWarp& epi = reinterpret_cast<EpiWarp*>(smem + C::EPI_OFF)[warp - 2];
@@ -676,10 +693,11 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (++s == C::STAGES) { s = 0; ph ^= 1u; fresh = false; }
             }
         }
+        if (rank == 0) drain_copies<C::STAGES>(full, s, ph, fresh);       // what both have brought in
     } else if (warp == 1) {
         int s = 0;
         uint32_t ph = 0, n = 0;
-        bool ok = rank == 0;
+        bool fresh = true, ok = rank == 0;
         for (int64_t tile = first; tile < tiles && ok; tile += step, ++n) {
             const uint32_t buf = n & 1u;
             if (n >= 2) ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[buf], ((n >> 1) & 1u) ^ 1u, DEVERR_PART_WAIT));
@@ -696,9 +714,10 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     umma2_commit(&empty[s]);
                     if (kb == kblocks - 1) umma2_commit(&acc_full[buf]);
                 }
-                if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+                if (++s == C::STAGES) { s = 0; ph ^= 1u; fresh = false; }
             }
         }
+        drain_mmas<C::STAGES>(empty, s, ph, fresh);                       // rank 1 has issued none
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         EpiWarp& epi = reinterpret_cast<EpiWarp*>(smem + C::EPI_OFF)[warp - 2];
@@ -794,6 +813,7 @@ int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
         grid_wait();
         int s = 0;
         uint32_t ph = 0;
+        bool first = true;
         for (int i = 0; i < nkb; ++i) {
             if (i >= C::STAGES) {
                 ok = __all_sync(0xffffffffu, mbar_wait_inline(&empty[s], ph ^ 1u, DEVERR_EMPTY_WAIT));
@@ -807,11 +827,13 @@ int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 }
                 tma_load_2d(st, &map_a, (kb0 + i) * IKB, m0, &full[s]);
             }
-            if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+            if (++s == C::STAGES) { s = 0; ph ^= 1u; first = false; }
         }
+        drain_copies<C::STAGES>(full, s, ph, first);
     } else if (warp == 1) {
         int s = 0;
         uint32_t ph = 0;
+        bool first = true;
         for (int i = 0; i < nkb; ++i) {
             ok = __all_sync(0xffffffffu, mbar_wait_inline(&full[s], ph, DEVERR_FULL_WAIT));
             if (!ok) break;
@@ -825,8 +847,9 @@ int8_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_consta
                 umma_commit(&empty[s]);
                 if (i == nkb - 1) umma_commit(done);
             }
-            if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+            if (++s == C::STAGES) { s = 0; ph ^= 1u; first = false; }
         }
+        drain_mmas<C::STAGES>(empty, s, ph, first);
     }
     grid_wait();                                             // the scales of the tokens come from the kernel before, too
     // the sums are complete (S > 1: and the stages free for them)
