@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(V == 1 ? kPairOneMaxN / 8 : kPairMaxThreads, 1
             sum = cta_sum2<W>(part1, part2, sums[par]);
             par ^= 1;
             // behind that barrier every thread has read the stage of the row whose pass 2 came before it
-            if (t == 0 && at2.j + S < end) fetch(done);
+            if (t == 0 && !dead && at2.j + S < end) fetch(done);      // a barrier whose copies did not come is not armed again
             fetch_scalars();
             pass3(scal[sc3], sum.y * p.inv_n, u, do_row);
             if (!more) break;
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(V == 1 ? kPairOneMaxN / 8 : kPairMaxThreads, 1
             fetch_scalars();
             copies_wait<0>();
             sum = cta_sum2<W>(part, 0.f, sums[1]);
-            if (t == 0 && at2.j + 1 < end) fetch(0);
+            if (t == 0 && !dead && at2.j + 1 < end) fetch(0);
             pass3(scal[sc], sum.x * p.inv_n, u, do_row);
             if (at2.j + 1 == end) break;
             next_row();
@@ -522,6 +522,10 @@ __global__ void __launch_bounds__(V == 1 ? kPairOneMaxN / 8 : kPairMaxThreads, 1
             ph ^= 1u;
             mbar_wait_or_mark<true>(&full[0], ph, DEVERR_FULL_WAIT, dead);
         }
+    }
+    if (t == 0 && dead) {    // rows that the wait gave up on may still be on their way to this CTA's shared memory: one more time limit
+        const int fetched = ahead.j - begin;
+        for (int i = max(0, fetched - S); i < fetched; ++i) mbar_wait_inline(&full[i % S], uint32_t(i / S) & 1u, DEVERR_FULL_WAIT);
     }
     grid_go();
     copies_wait<0>();

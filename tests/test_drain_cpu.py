@@ -1,4 +1,4 @@
-"""The issuing warps of the int8 product's kernels leave when their copies and MMAs are complete, also behind a wait that gave up: which
+"""The issuing threads of the 8-bit operators' pipelined kernels leave when their copies and MMAs are complete, also behind a wait that gave up: which
 uses of the ring's barriers they wait for, by a model of the barriers, and that every kernel does so."""
 
 import os
@@ -42,3 +42,14 @@ def test_every_kernel_waits():
         assert "drain_mmas<C::STAGES>(empty, s, ph, " in rest
         # the flag of the first pass falls where the stage wraps
         assert len(re.findall(r"if \(\+\+s == C::STAGES\) \{ s = 0; ph \^= 1u; (?:first|fresh) = false; \}", body)) == 2
+
+
+def test_the_ring_of_rows():
+    """The norm pair's gradient fetches no row once its wait has given up, and then waits for the rows on their way."""
+    with open(os.path.join(os.path.dirname(SOURCE), "lh_pair.cu")) as fh:
+        text = fh.read()
+    body = text[text.index("pair_bwd_kernel(const PairParams p)"):text.index("pair_reduce_kernel(")]
+    in_loops = body[body.index("bool dead = false;"):]
+    assert len(re.findall(r"\bfetch\(", in_loops)) == len(re.findall(r"if \(t == 0 && !dead && .*\) fetch\(", in_loops)) == 2
+    assert re.search(r"if \(t == 0 && dead\) \{.*?\n.*?\n +for \(int i = max\(0, fetched - S\); i < fetched; \+\+i\) "
+                     r"mbar_wait_inline\(&full\[i % S\], uint32_t\(i / S\) & 1u, DEVERR_FULL_WAIT\);", in_loops)
