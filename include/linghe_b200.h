@@ -358,8 +358,8 @@ int lh_fp8_gemm_bb(const void* a, const void* b, const float* a_s, const float* 
  * (0 = none).  A checkpoint of a [M, n] tensor is its codes [M, n] and one float32 scale per 1x128 block,
  * row-major [M, n/128] (the layout of lh_group_quant, whose outputs are a checkpoint of format 2):
  *   scale = max(amax / top, 1e-30), top = 127 or 448;   code = nearest(x / scale), ties to even.
- * A block with a NaN or an infinity has a NaN scale.  All pointers 16-byte aligned but those of scales, sums and
- * per-row values. */
+ * A block with a NaN or an infinity has a NaN scale.  All pointers 16-byte aligned, the smoothing factors' too, but those of
+ * scales (os, hs, s, a_s, b_s), sums (dpost, dpre) and per-row values (r_post, r_pre, w, dw): those lie anywhere. */
 
 /* The norm after a block, its gate and residual scale, the residual sum and the norm before the next block:
  *   r_post = rsqrt(mean(o^2) + eps);  h = round(x + alpha * gate * (o * r_post * post));
@@ -393,7 +393,7 @@ int lh_silu_checkpoint_bwd(const void* g, const void* q, const float* s, const v
                            int codes, int64_t M, int64_t n, void* dx, void* dw, void* stream);
 
 /* One float32 scale per row and int8 codes: x [M,K] of `dtype`, K % 16 == 0;
- *   xs = x / max(smooth, 1e-30) (smooth float32 [K] or NULL);  s[m] = max(amax_k |xs| / 127, 1e-30);
+ *   xs = x / max(smooth, 1e-30) (smooth float32 [K], 16-byte aligned, or NULL);  s[m] = max(amax_k |xs| / 127, 1e-30);
  *   q = nearest(xs / s), ties to even.  A row with a NaN or an infinity has a NaN scale. */
 int lh_token_quant_int8(const void* x, const float* smooth, int dtype, int64_t M, int64_t K, void* q, float* s,
                         void* stream);

@@ -41,7 +41,8 @@ def int8_linear(x, w, w_s, smooth_scale=None, out_dtype=None):
     """x @ dequant(w).T for `x` [..., K] (bf16, fp16 or fp32), quantised per token on the way, and int8 weights `w`
     [N, K] with one float32 scale `w_s` [N] per output channel: `token_quant_int8` and `int8_gemm` in one call.
 
-    `smooth_scale` (float32 [K]): x is divided by it before it is quantised; the weights hold the product with it.
+    `smooth_scale` (float32 [K], at a 16-byte boundary like x): x is divided by it before it is quantised; the
+    weights hold the product with it.
     The result has `out_dtype`, that of x by default.  There is no backward pass: an x, w_s or smooth_scale that requires a
     gradient is refused unless the call is under torch.no_grad()."""
     host = _lib.host()

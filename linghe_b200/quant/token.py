@@ -10,8 +10,8 @@ from linghe_b200 import _lib
 def token_quant_int8(x, smooth_scale=None, out=None, scale=None):
     """One float32 scale per row and int8 codes of `x` [..., K] (bf16, fp16 or fp32; K % 16 == 0).
 
-    With `smooth_scale` (float32 [K]) the row is divided by max(smooth_scale, 1e-30) first, as in the smooth
-    quantisers of this package.  scale = max(amax / 127, 1e-30), code = nearest(x / scale), ties to even; a row
+    With `smooth_scale` (float32 [K], at a 16-byte boundary like x) the row is divided by max(smooth_scale, 1e-30)
+    first, as in the smooth quantisers of this package.  scale = max(amax / 127, 1e-30), code = nearest(x / scale), ties to even; a row
     with a NaN or an infinity gets a NaN scale.  Weights [N, K] take the same call: one scale per output channel.
     Returns (out int8 like x, scale float32 [rows])."""
     host = _lib.host()
