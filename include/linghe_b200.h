@@ -384,7 +384,8 @@ int lh_rmsnorm_pair_bwd(const void* dy, const void* dh, const void* o, const flo
 
 /* SwiGLU that keeps an 8-bit checkpoint of its input: y [M,n] = silu(x1) * x2 [* w_row] of `dtype` and the
  * checkpoint (q [M,2n], s [M,2n/128]) of x [M,2n].  codes 1 or 2; w NULL or [M] in w_dtype (LH_F32 / LH_BF16);
- * n % 128 == 0. */
+ * n % 128 == 0.  The sigmoid is float32 from a base-2 exponential: a relative error of up to (|x1| + 64) * 2^-24, and 0
+ * where it is below the normal numbers (x1 < -87), here and in the gradient. */
 int lh_silu_checkpoint_fwd(const void* x, const void* w, int dtype, int w_dtype, int codes, int64_t M, int64_t n,
                            void* y, void* q, float* s, void* stream);
 

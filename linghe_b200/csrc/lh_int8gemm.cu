@@ -23,7 +23,8 @@ constexpr int64_t kInt8MaxK = 131071 / 16 * 16;
 // ---- token-wise quantiser ---------------------------------------------------------------------
 // A team of warps takes a row, a lane 32 bytes of it.  Rows that 16 warps hold that way (HOLD: 8192 elements of a 16-bit
 // type, 4096 of float32) stay in registers between the maximum and the codes, longer ones are walked twice, the second
-// time through L2.  Small registers, so that six rows of 4096 are in flight on an SM: that is what it waits for.
+// time through L2.  Small registers, so that six rows of 4096 are in flight on an SM: that is what it waits for (8192 x 4096 bf16
+// 24.0 us, floor 15.4; smoothed, with a division per element, 42.4; float32 41.6, floor 25.6).
 constexpr int kTokWarps = 16;
 
 struct TokenParams {
@@ -201,7 +202,9 @@ __device__ __forceinline__ void fetch_scales(const Int8Params& p, int n0, int co
 // per step straight into the fragments of mma.m16n8k32 (k may be in any order as long as both operands agree, so
 // a lane's 16 consecutive bytes serve as the two 4-byte pieces of two instructions).  Eight tokens fill the n = 8 of
 // the instruction; NT such groups.  The weights are asked for before the wait for the kernel that writes the codes.  64 registers,
-// so that two CTAs of 16 warps are on an SM: 1 x 4096 x 4096 4.2 us (4.0 TB/s; 5.5 us with one), 1 x 8192 x 8192 14.7 us (4.6 TB/s).
+// so that two CTAs of 16 warps are on an SM.  bf16 results, weights from HBM (sets of them in turn that exceed L2): 1 x 4096 x 4096
+// 5.9 us (floor 2.6), 8 x 4096 x 4096 6.3, 1 x 8192 x 8192 14.4 (floor 10.3), 4 x 4096 x 14336 13.8 (floor 9.0); weights in L2: 1 x
+// 4096 x 4096 4.1, 5.5 with one CTA on an SM.  A warp has four steps in flight and asks for the next four when it has used them.
 constexpr int kRowsSteps = 4;      // steps of a warp in flight
 
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -288,7 +291,8 @@ __global__ void __launch_bounds__(512, NT == 1 ? 2 : 1) int8_rows_kernel(const I
 
 // One token with the quantiser inside: every CTA makes the token's codes itself (from L2, while its weights are on their way).
 // As long as all CTAs run at once that costs about what the kernel in front does, and the second launch is saved: one token
-// through 4096 x 4096 takes 5.5 us on the GPU either way and 0.5 us less a call, through 1024 x 1024 3.8 us.  With more
+// through 4096 x 4096 (bf16) takes 5.5 us on the GPU either way and 0.5 us less a call with the weights in L2 (7.1 us from HBM),
+// through 1024 x 1024 3.8 us.  With more
 // tokens or channels the repeated work is longer than the launch (6 x 8192 x 2048: 14 us, 5.5 in two kernels).
 // The arithmetic is that of token_quant_kernel; CTA 0 leaves codes and scale in the workspaces.
 constexpr int kFusedMaxK = 16384;
@@ -437,8 +441,9 @@ __device__ __forceinline__ void drain_mmas(uint64_t* empty, int s, uint32_t ph, 
 }
 
 // Products of many tiles and little k: one persistent CTA per SM walks tiles (column tile fastest); warp 0 TMA, warp 1 MMA,
-// warps 2-9 read the sums of the tile before out of the other tensor-memory buffer, scale and store them.  Twice as many CTAs
-// store as in the kernel for pairs of SMs below, which is ahead otherwise (4096 x 8192 x 512: 30 us, 39 there).
+// warps 2-9 read the sums of the tile before out of the other tensor-memory buffer, scale and store them.  A tile has a quarter of the
+// sums of one of the kernel for pairs of SMs below: ahead where k is short (4096 x 8192 x 512 bf16 30 us, 34 there), far behind
+// where it is long (8192 x 8192 x 4096 266 us, 177 there).
 template <int TN>
 struct BigTile {
     static constexpr int STAGE = I_ATILE + TN * IKB;
@@ -555,8 +560,8 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 
 // The largest products: two CTAs of a cluster (a pair of SMs) share a 256 x 256 tile, tcgen05.mma.cta_group::2.  Each
 // brings in its 128 rows of a and its 128 rows of b, half of what the pair multiplies, so an SM takes 32 KB per 128 bytes of k
-// for 128 x 256 sums; a CTA alone takes 48, 96 bytes per cycle at the full rate of the tensor cores, more than L2 gives (8192 x
-// 8192 x 4096: 201 us against 178, 8192^3: 485 against 364).  From about 4096 of k on the power limit bounds it: 0.40 us per 128
+// for 128 x 256 sums; a CTA alone takes 48, 96 bytes per cycle at the full rate of the tensor cores, more than L2 gives (bf16
+// results, 8192 x 8192 x 4096: 201 us against 178, 8192^3: 485 against 364).  From about 4096 of k on the power limit bounds it: 0.40 us per 128
 // of k where a short run takes 0.26; below 1024 of k the stores do, about 5 us per tile.  The leader (rank 0) issues for both; full[] counts in the leader's shared memory what both
 // bring, commits arrive in both CTAs, both read their half of the sums.
 struct PairTile {
@@ -754,8 +759,9 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 // Products of few tiles: a cluster of S CTAs shares k of one tile; the rank is the part of k.  Rank r owns the rows r, r + S,
 // ... of the tile: every CTA writes its sums of them to its own place in the owner's shared memory (stores to the other
 // SMs that nobody waits for; reading them from there instead took twice as long), and behind one cluster barrier the
-// owner adds them up and stores the result.  What bounds it is the issue of the MMAs, four per 128 bytes of k whatever
-// their size (about 0.28 us), so k is split as far as there are SMs.
+// owner adds them up and stores the result.  What bounds it is the step of the warp that issues the MMAs (wait, four MMAs, commit),
+// 0.27 us per 128 bytes of k: a CTA alone on the GPU takes that with 3 to 7 stages and 64 columns (0.29 with 128, and with 2 stages),
+// 0.27 still without its loads, 0.22 without its MMAs; with 128 CTAs 0.29 and 0.34.  So k is split as far as there are SMs.
 template <int TN>
 struct SplitTile {
     static constexpr int STAGE = I_ATILE + TN * IKB;
@@ -1028,10 +1034,11 @@ int int8_product(Int8Params p, bool dependent, cudaStream_t stream) {
     };
     // Which kernel, by an estimate in microseconds: the slowest CTA's MMAs per 128 bytes of k, at least its stores, or what all
     // CTAs bring in through L2 at 9.5 TB/s, and what follows the last MMA: the join of a split k, or stores that nothing hides (longest
-    // where rows have to be written element by element).  It follows the measured times within about 2 us plus 4 for
-    // the launch: 32 x 4096 x 4096 8.2 us (128 columns, k in 4; whole 15.1), 300 x 1024 x 8192 13.7 (in 4; 25.0),
-    // 1000 x 1111 x 2064 12.3 (64 columns, whole; 128 columns in 2 14.4), 512 x 4096 x 4096 16.6 (pair; 128 columns 18.1),
-    // 4096 x 8192 x 512 34 (tile; pair 39), 8192 x 8192 x 4096 180 (pair; tile 285).
+    // where rows have to be written element by element).  Plus 4 for the launch it follows the measured times within 3 us in most cases
+    // (bf16 results): 32 x 4096 x 4096 8.3 us (128 columns, k in 4; whole 15.1), 300 x 1024 x 8192 13.7 (128 columns, in 4;
+    // 64 in 2 15.7; whole 24.6), 4096 x 8192 x 512 30 (tile; pair 34), 8192 x 8192 x 4096 177 (pair; tile 266).  Where it is wrong:
+    // 1000 x 1111 x 2064 14.4 (128 columns, in 2; 64 columns, whole, 12.4), 512 x 4096 x 4096 16.4 (pair; 128 columns 17.8; tile,
+    // which is not considered for so few tiles, 14.5).
     const int kblocks = int(ceil_div(p.K, IKB));
     enum { SPLIT64, SPLIT128, TILE, PAIR };
     int kind = PAIR, parts = 1;
