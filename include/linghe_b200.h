@@ -376,7 +376,7 @@ int lh_rmsnorm_pair_fwd(const void* x, const void* o, const void* post, const vo
  * tensors of the forward pass (codes 0), or their checkpoints with scales os, hs.  r_post, r_pre from the forward pass.
  * Writes dx = the gradient of x and of h's other use, dout = that of o [M, n]; dpost, dpre float32 [n]; dgate [G, n]
  * of `dtype` (gate != NULL).  Sums over rows are float32 in a fixed order: equal calls give equal bits.
- * scratch: lh_scratch_bytes("rmsnorm_pair_bwd", M, n) bytes.  M = 0 gives zero sums. */
+ * scratch: lh_scratch_bytes("rmsnorm_pair_bwd", M, n) bytes (0 for sizes that are refused).  M = 0 gives zero sums. */
 int lh_rmsnorm_pair_bwd(const void* dy, const void* dh, const void* o, const float* os, const void* h, const float* hs,
                         const void* post, const void* pre, const void* gate, const float* r_post, const float* r_pre,
                         int dtype, int64_t M, int64_t n, int64_t G, float alpha, int codes, void* dx, void* dout,

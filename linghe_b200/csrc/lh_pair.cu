@@ -718,7 +718,7 @@ int pair_check(const char* what, int dtype, int64_t M, int64_t n, const void* ga
 }  // namespace
 
 int64_t pair_bwd_scratch(int64_t M, int64_t n) {
-    if (M <= 0 || n <= 0 || n > kPairMaxN) return 0;
+    if (M <= 0 || n <= 0 || n > kPairMaxN || (n % 128) != 0) return 0;     // sizes that the call refuses (or has nothing to do for)
     return pair_bwd_grid(M, n) * PART_ROWS * n * 4;
 }
 
