@@ -5,6 +5,8 @@ import sys
 
 import pytest
 
+from linghe_b200 import _lib
+
 KINDS = ["rmsnorm_bwd", "batch_silu_bwd", "smooth_quant", "smooth_quant_bwd", "row_id_map", "rmsnorm_pair_bwd", "rmsnorm_gemm", "none of them"]
 
 
@@ -12,11 +14,12 @@ KINDS = ["rmsnorm_bwd", "batch_silu_bwd", "smooth_quant", "smooth_quant_bwd", "r
 def test_any_sizes(kind):
     """In a process of its own, which an integer division by zero would end."""
     code = f"""
-from linghe_b200 import _lib
-lib = _lib.load()
+import ctypes
+size = ctypes.CDLL({_lib.LIB_PATH!r}).lh_scratch_bytes
+size.restype, size.argtypes = ctypes.c_int64, [ctypes.c_char_p, ctypes.c_int64, ctypes.c_int64]
 for rows in (-1, 0, 1, 4, 1 << 20, (1 << 31) - 1):
     for cols in (-128, -1, 0, 1, 8, 15, 16, 31, 100, 128, 200, 4096, 5120, 8192, 8320, 1 << 20):
-        v = lib.lh_scratch_bytes({kind!r}.encode(), rows, cols)
+        v = size({kind!r}.encode(), rows, cols)
         if {kind!r} == "rmsnorm_pair_bwd":
             assert (v > 0) == (rows > 0 and cols in (128, 4096, 5120, 8192)), (rows, cols, v)
 print("done")
