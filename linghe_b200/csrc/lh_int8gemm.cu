@@ -561,7 +561,7 @@ int8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 // The largest products: two CTAs of a cluster (a pair of SMs) share a 256 x 256 tile, tcgen05.mma.cta_group::2.  Each
 // brings in its 128 rows of a and its 128 rows of b, half of what the pair multiplies, so an SM takes 32 KB per 128 bytes of k
 // for 128 x 256 sums; a CTA alone takes 48, 96 bytes per cycle at the full rate of the tensor cores, more than L2 gives (bf16
-// results, 8192 x 8192 x 4096: 201 us against 178, 8192^3: 485 against 364).  From about 4096 of k on the power limit bounds it: 0.40 us per 128
+// results, 8192 x 8192 x 4096: 201 us against 177, 8192^3: 485 against 364 to 379, by the card).  From about 4096 of k on the power limit bounds it: 0.40 us per 128
 // of k where a short run takes 0.26; below 1024 of k the stores do, about 5 us per tile.  The leader (rank 0) issues for both; full[] counts in the leader's shared memory what both
 // bring, commits arrive in both CTAs, both read their half of the sums.
 struct PairTile {
